@@ -372,6 +372,45 @@ QSA_API int qsa_sparse_attention_static_scratch(
     int64_t out_head_stride, int32_t indices_are_physical, int32_t use_decode_kernel,
     void* stream);
 
+/* Element types of the entry points below that take one. */
+enum qsa_dtype { QSA_DTYPE_BF16 = 0, QSA_DTYPE_F16 = 1, QSA_DTYPE_F32 = 2 };
+
+/*
+ * Rotary positions of query and key heads, with the optional store of keys and
+ * values to the paged cache, one launch.  No counterpart in the reference's
+ * operators: its layer rotates the main queries and keys before they reach
+ * qsa_prepare.
+ *
+ * For every token t, head and pair i < rotary_dim / 2, with
+ * a = positions[t] * frequencies[i] (radians, formed and reduced in 64 bits):
+ *   y1 = factor * (x1 cos a - x2 sin a),  y2 = factor * (x2 cos a + x1 sin a)
+ * (x1, x2) = (x[i], x[i + rotary_dim / 2]), or (x[2i], x[2i + 1]) when
+ * interleaved; dims from rotary_dim on are copied.  32-bit products, one
+ * rounding.  inverse negates the sine: with the same factor that is the
+ * transposed map, which takes the gradient of y to the gradient of x.
+ * q [num_tokens, num_q_heads, head_dim] goes to q_out, k [num_tokens,
+ * num_kv_heads, head_dim] to k_out (q_out / k_out may be q / k with the same
+ * strides; any other overlap is the caller's error).  With slots (int64
+ * [num_tokens], stride slots_stride) keys and v go to k_cache / v_cache
+ * [num_blocks, page_size, num_kv_heads, head_dim] instead and k_out is
+ * ignored: slot page*page_size+offset; slots < 0 are skipped, slots past the
+ * cache are skipped and set QSA_DEVICE_ERR_OUT_OF_RANGE.  A head count of 0
+ * leaves that side out.  All of one dtype (QSA_DTYPE_*), unit dim strides;
+ * other strides in elements.  positions: int64; frequencies: double
+ * [rotary_dim / 2], on the device.  head_dim 1..1024, rotary_dim even.
+ */
+QSA_API int qsa_rotary(
+    const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t num_q_heads, void* q_out,
+    int64_t q_out_row_stride, int64_t q_out_head_stride, const void* k, int64_t k_row_stride,
+    int64_t k_head_stride, int32_t num_kv_heads, void* k_out, int64_t k_out_row_stride,
+    int64_t k_out_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride,
+    void* k_cache, int64_t k_block_stride, int64_t k_token_stride, int64_t k_cache_head_stride,
+    void* v_cache, int64_t v_block_stride, int64_t v_token_stride, int64_t v_cache_head_stride,
+    int64_t num_blocks, int32_t page_size, const int64_t* slots, int64_t slots_stride,
+    int32_t num_tokens, int32_t head_dim, const int64_t* positions, int64_t positions_stride,
+    const double* frequencies, int32_t rotary_dim, float factor, int32_t interleaved,
+    int32_t inverse, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

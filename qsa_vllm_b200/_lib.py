@@ -58,6 +58,10 @@ SIGNATURES: dict[str, tuple] = {
         _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64,
         _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64,
         _i64, _i32, _vp, _i32, _i32, _vp]),
+    "qsa_rotary": (C.c_int, [
+        _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64,
+        _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64,
+        _i32, _i32, _vp, _i64, C.c_void_p, _i32, _f32, _i32, _i32, _i32, _vp]),
     "qsa_sparse_attention_static_scratch": (C.c_int, [
         _vp, _i64, _i64, _i32, _i32, _i32,
         _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32,
@@ -109,6 +113,26 @@ def ensure_device(device: torch.device) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    """A context that changes nothing (the tensors' device is the current one)."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, free of charge when it is the current one already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

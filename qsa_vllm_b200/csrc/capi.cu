@@ -618,6 +618,112 @@ int qsa_prepare(const void* index_qk, int64_t index_row_stride, int32_t num_toke
   return QSA_OK;
 }
 
+// ----------------------------------------------------------------- rotary
+int qsa_rotary(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t num_q_heads,
+               void* q_out, int64_t q_out_row_stride, int64_t q_out_head_stride, const void* k,
+               int64_t k_row_stride, int64_t k_head_stride, int32_t num_kv_heads, void* k_out,
+               int64_t k_out_row_stride, int64_t k_out_head_stride, const void* v,
+               int64_t v_row_stride, int64_t v_head_stride, void* k_cache, int64_t k_block_stride,
+               int64_t k_token_stride, int64_t k_cache_head_stride, void* v_cache,
+               int64_t v_block_stride, int64_t v_token_stride, int64_t v_cache_head_stride,
+               int64_t num_blocks, int32_t page_size, const int64_t* slots, int64_t slots_stride,
+               int32_t num_tokens, int32_t head_dim, const int64_t* positions,
+               int64_t positions_stride, const double* frequencies, int32_t rotary_dim,
+               float factor, int32_t interleaved, int32_t inverse, int32_t dtype, void* stream) {
+  const char* who = "qsa_rotary";
+  if (num_tokens < 0 || num_q_heads < 0 || num_kv_heads < 0)
+    return fail(QSA_ERR_INVALID, "%s: negative size", who);
+  if (dtype != QSA_DTYPE_BF16 && dtype != QSA_DTYPE_F16 && dtype != QSA_DTYPE_F32)
+    return fail(QSA_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
+  if (head_dim <= 0 || head_dim > 1024)
+    return fail(QSA_ERR_UNSUPPORTED, "%s: head_dim %d (1..1024 supported)", who, head_dim);
+  if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim)
+    return fail(QSA_ERR_INVALID, "%s: rotary dim %d must be even and in [2, %d]", who, rotary_dim,
+                head_dim);
+  if (static_cast<int64_t>(num_q_heads) + 2 * static_cast<int64_t>(num_kv_heads) > 65536)
+    return fail(QSA_ERR_UNSUPPORTED, "%s: more than 65536 heads", who);
+  if (num_tokens == 0 || (num_q_heads == 0 && num_kv_heads == 0)) return QSA_OK;
+  if (!positions || !frequencies || (num_q_heads > 0 && (!q || !q_out)) ||
+      (num_kv_heads > 0 && !k))
+    return fail(QSA_ERR_INVALID, "%s: null pointer", who);
+  const bool store = slots != nullptr;
+  if (num_kv_heads > 0) {
+    if (store ? (!v || !k_cache || !v_cache) : !k_out)
+      return fail(QSA_ERR_INVALID, "%s: null key / value destination", who);
+    if (store && (page_size <= 0 || num_blocks < 0))
+      return fail(QSA_ERR_INVALID, "%s: bad page geometry", who);
+  }
+  const int64_t size = dtype == QSA_DTYPE_F32 ? 4 : 2, chunk = 16 / size;
+  const void* ptrs[] = {q, q_out, k, store ? k_cache : k_out, v, v_cache};
+  const bool used[] = {num_q_heads > 0, num_q_heads > 0, num_kv_heads > 0, num_kv_heads > 0,
+                       num_kv_heads > 0 && store, num_kv_heads > 0 && store};
+  const int64_t strides[][3] = {
+      {q_row_stride, q_head_stride, 0}, {q_out_row_stride, q_out_head_stride, 0},
+      {k_row_stride, k_head_stride, 0},
+      {store ? k_block_stride : k_out_row_stride, store ? k_token_stride : 0,
+       store ? k_cache_head_stride : k_out_head_stride},
+      {v_row_stride, v_head_stride, 0}, {v_block_stride, v_token_stride, v_cache_head_stride}};
+  // the pairs' halves, and the dims past them, in whole chunks
+  bool vec = head_dim % chunk == 0 && rotary_dim % (interleaved ? chunk : 2 * chunk) == 0;
+  for (int i = 0; i < 6; ++i) {
+    if (!used[i]) continue;
+    if (!aligned(ptrs[i], size))
+      return fail(QSA_ERR_INVALID, "%s: a tensor is not aligned to its elements", who);
+    vec = vec && aligned(ptrs[i], 16) && strides[i][0] % chunk == 0 && strides[i][1] % chunk == 0 &&
+          strides[i][2] % chunk == 0;
+  }
+  RotaryParams p = {};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_row_stride = q_row_stride;
+  p.q_head_stride = q_head_stride;
+  p.k_row_stride = k_row_stride;
+  p.k_head_stride = k_head_stride;
+  p.v_row_stride = v_row_stride;
+  p.v_head_stride = v_head_stride;
+  p.q_out = q_out;
+  p.k_out = k_out;
+  p.qo_row_stride = q_out_row_stride;
+  p.qo_head_stride = q_out_head_stride;
+  p.ko_row_stride = k_out_row_stride;
+  p.ko_head_stride = k_out_head_stride;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.kc_block_stride = k_block_stride;
+  p.kc_token_stride = k_token_stride;
+  p.kc_head_stride = k_cache_head_stride;
+  p.vc_block_stride = v_block_stride;
+  p.vc_token_stride = v_token_stride;
+  p.vc_head_stride = v_cache_head_stride;
+  p.num_blocks = num_blocks;
+  p.page_size = store && page_size > 0 ? page_size : 1;
+  p.page_div = FastDiv(static_cast<uint32_t>(p.page_size));
+  p.slots = slots;
+  p.slot_stride = slots_stride;
+  p.num_tokens = num_tokens;
+  p.q_heads = num_q_heads;
+  p.kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.positions = positions;
+  p.positions_stride = positions_stride;
+  p.frequencies = frequencies;
+  p.rotary_dim = rotary_dim;
+  p.factor = factor;
+  p.interleaved = interleaved ? 1 : 0;
+  p.inverse = inverse ? 1 : 0;
+  p.dtype = dtype;
+  p.vec = vec ? 1 : 0;
+  p.q_in_place = q == q_out && q_row_stride == q_out_row_stride &&
+                 q_head_stride == q_out_head_stride;
+  p.k_in_place = !store && k == k_out && k_row_stride == k_out_row_stride &&
+                 k_head_stride == k_out_head_stride;
+  p.err = device_error_word();
+  cudaError_t e = launch_rotary(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return QSA_OK;
+}
+
 // -------------------------------------------------------------- attention
 size_t qsa_sparse_attention_workspace_bytes(int32_t rows, int32_t num_q_heads,
                                             int32_t num_kv_heads, int32_t head_dim,

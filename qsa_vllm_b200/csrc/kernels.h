@@ -220,6 +220,37 @@ struct PrepareParams {
 };
 cudaError_t launch_prepare(const PrepareParams& p, cudaStream_t stream);
 
+// ---------------------------------------------------------------- rotary
+enum { kDtypeBF16 = 0, kDtypeF16 = 1, kDtypeF32 = 2 };  // the C ABI's qsa_dtype
+struct RotaryParams {
+  const void *q, *k, *v;   // [tokens, heads, dim], unit dim stride
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+  void *q_out, *k_out;     // k_out unused when slots are given
+  int64_t qo_row_stride, qo_head_stride, ko_row_stride, ko_head_stride;
+  void *k_cache, *v_cache; // [blocks, page, kv_heads, dim]
+  int64_t kc_block_stride, kc_token_stride, kc_head_stride;
+  int64_t vc_block_stride, vc_token_stride, vc_head_stride;
+  int64_t num_blocks;
+  int page_size;
+  FastDiv page_div;
+  const int64_t* slots;    // nullptr: no store
+  int64_t slot_stride;
+  int num_tokens, q_heads, kv_heads, head_dim;
+  const int64_t* positions;
+  int64_t positions_stride;
+  const double* frequencies;  // [rotary_dim / 2], radians per position
+  int rotary_dim;
+  float factor;
+  int interleaved, inverse, dtype;
+  int vec;                 // 16-byte chunks everywhere
+  int q_in_place, k_in_place;
+  // filled by launch_rotary: items of one token, and their division into heads
+  int q_items, k_items;
+  FastDiv item_div, q_head_div, k_head_div, v_head_div;
+  int* err;
+};
+cudaError_t launch_rotary(RotaryParams p, cudaStream_t stream);
+
 int num_sms();
 // One CTA waits on an mbarrier phase nothing completes; the bounded wait
 // expires and records kDeviceErrWaitTimeout in *err (selftest.cu).
