@@ -411,6 +411,70 @@ QSA_API int qsa_rotary(
     const double* frequencies, int32_t rotary_dim, float factor, int32_t interleaved,
     int32_t inverse, int32_t dtype, void* stream);
 
+/*
+ * Compaction of cached tokens.  No counterpart in the reference.
+ *
+ * For every request b, KV head h and j < count with indices[b, h, j] >= 0, the
+ * key and value rows of logical token indices[b, h, j] go to logical token
+ * starts[b] + j (starts NULL: j).  Entries below 0 move nothing.  Tokens are
+ * found through block_table [num_requests, table_width]; destinations through
+ * out_table, or block_table again when out_table is NULL (in place).
+ * In place each list must be strictly ascending over its entries that are not
+ * below 0, and no source may lie below its destination.  With an out_table,
+ * destinations must not be pages that the call also reads.
+ * Entries outside the tables or on unmapped pages, and in-place sources below
+ * their destination, are skipped and set QSA_DEVICE_ERR_OUT_OF_RANGE.
+ * indices: int32, unit stride over j; a head stride of 0 shares one list.
+ * Caches as in qsa_sparse_attention, of any QSA_DTYPE_*; rows of any
+ * alignment (16-byte rows move fastest).  num_requests * num_kv_heads at most
+ * 65535.
+ */
+QSA_API int qsa_cache_compact(
+    void* k_cache, int64_t k_block_stride, int64_t k_token_stride, int64_t k_head_stride,
+    void* v_cache, int64_t v_block_stride, int64_t v_token_stride, int64_t v_head_stride,
+    int64_t num_blocks, int32_t page_size, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+    const int32_t* block_table, int64_t table_row_stride, int32_t table_width,
+    const int32_t* out_table, int64_t out_table_row_stride, int32_t out_table_width,
+    int32_t num_requests, const int32_t* indices, int64_t indices_request_stride,
+    int64_t indices_head_stride, int32_t count, const int32_t* starts, void* stream);
+
+/* Workspace bytes of qsa_cache_evict (0 for shapes it rejects). */
+QSA_API size_t qsa_cache_evict_workspace_bytes(int32_t num_requests, int32_t list_heads,
+                                               int32_t budget, int32_t sinks, int32_t recent);
+
+/*
+ * Eviction from the cache by accumulated attention weight.  No counterpart in
+ * the reference.
+ *
+ * Per request b with L = min(seq_lens[b], capacity) cached tokens and per list
+ * head h: all tokens when L <= budget; else the first `sinks`, the last
+ * `recent`, and of those between the budget - sinks - recent with the largest
+ * weights (ties to the lowest token; fp32 bit patterns as unsigned numbers are
+ * compared, so weights are expected to be 0 or above; a NaN counts as largest).
+ * The kept tokens, ascending, become tokens 0 .. min(L, budget) - 1: their K/V
+ * rows move as qsa_cache_compact moves them (in place, or to out_table's
+ * pages), weights_out[b, h, j] = weights[b, h, kept[j]], zero from there to L
+ * (entries from L on are not written).  kept [num_requests, list_heads,
+ * budget] receives the old token numbers, -1 behind the last; lengths_out
+ * [num_requests] the new lengths.  seq_lens is not written, and neither
+ * weights_out unless it is weights may overlap what the call reads.
+ * weights: fp32 [num_requests, list_heads, capacity], unit token stride,
+ * (request, head) rows evenly spaced; list_heads = num_kv_heads, or 1 for a
+ * list shared by all heads.  Up to topk limits (see qsa_topk): capacity -
+ * sinks - recent <= 524288, budget - sinks - recent <= 49152.
+ */
+QSA_API int qsa_cache_evict(
+    const float* weights, int64_t weights_request_stride, int64_t weights_head_stride,
+    int32_t list_heads, int32_t capacity, const int32_t* seq_lens, int32_t num_requests,
+    int32_t budget, int32_t sinks, int32_t recent, void* k_cache, int64_t k_block_stride,
+    int64_t k_token_stride, int64_t k_head_stride, void* v_cache, int64_t v_block_stride,
+    int64_t v_token_stride, int64_t v_head_stride, int64_t num_blocks, int32_t page_size,
+    int32_t num_kv_heads, int32_t head_dim, int32_t dtype, const int32_t* block_table,
+    int64_t table_row_stride, int32_t table_width, const int32_t* out_table,
+    int64_t out_table_row_stride, int32_t out_table_width, float* weights_out,
+    int64_t weights_out_request_stride, int64_t weights_out_head_stride, int32_t* kept,
+    int32_t* lengths_out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -62,6 +62,14 @@ SIGNATURES: dict[str, tuple] = {
         _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64,
         _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64,
         _i32, _i32, _vp, _i64, C.c_void_p, _i32, _f32, _i32, _i32, _i32, _vp]),
+    "qsa_cache_compact": (C.c_int, [
+        _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+        _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _i32, _vp, _vp]),
+    "qsa_cache_evict_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "qsa_cache_evict": (C.c_int, [
+        _vp, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _i32,
+        _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+        _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
     "qsa_sparse_attention_static_scratch": (C.c_int, [
         _vp, _i64, _i64, _i32, _i32, _i32,
         _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _i32,

@@ -724,6 +724,194 @@ int qsa_rotary(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32
   return QSA_OK;
 }
 
+// ------------------------------------------------------------ cache moves
+// The caches, tables and copy width of a move; a status other than QSA_OK has
+// its message set.
+static int move_common(MoveParams& p, const char* who, void* k_cache, int64_t k_block_stride,
+                       int64_t k_token_stride, int64_t k_head_stride, void* v_cache,
+                       int64_t v_block_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       int64_t num_blocks, int32_t page_size, int32_t num_kv_heads,
+                       int32_t head_dim, int32_t dtype, const int32_t* block_table,
+                       int64_t table_stride, int32_t table_width, const int32_t* out_table,
+                       int64_t out_table_stride, int32_t out_table_width, int32_t requests) {
+  if (dtype != QSA_DTYPE_BF16 && dtype != QSA_DTYPE_F16 && dtype != QSA_DTYPE_F32)
+    return fail(QSA_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
+  if (requests < 0 || num_kv_heads <= 0 || head_dim <= 0 || page_size <= 0 || num_blocks < 0 ||
+      table_width < 0 || out_table_width < 0)
+    return fail(QSA_ERR_INVALID, "%s: bad sizes", who);
+  if (static_cast<int64_t>(requests) * num_kv_heads > 65535)
+    return fail(QSA_ERR_UNSUPPORTED, "%s: %d requests x %d heads exceed 65535", who, requests,
+                num_kv_heads);
+  if (requests == 0) return QSA_OK;
+  if (!k_cache || !v_cache || !block_table) return fail(QSA_ERR_INVALID, "%s: null pointer", who);
+  const int64_t size = dtype == QSA_DTYPE_F32 ? 4 : 2;
+  const int64_t bytes[] = {k_block_stride * size, k_token_stride * size, k_head_stride * size,
+                           v_block_stride * size, v_token_stride * size, v_head_stride * size,
+                           head_dim * size};
+  if (!aligned(k_cache, size) || !aligned(v_cache, size))
+    return fail(QSA_ERR_INVALID, "%s: a cache is not aligned to its elements", who);
+  int64_t unit = 16;
+  for (const void* c : {k_cache, v_cache})
+    while (!aligned(c, unit)) unit /= unit == 16 ? 4 : 2;
+  for (const int64_t n : bytes)
+    while (n % unit) unit /= unit == 16 ? 4 : 2;
+  if (bytes[6] / unit > move_max_row_units())
+    return fail(QSA_ERR_UNSUPPORTED, "%s: rows of %lld units of %lld bytes exceed %d", who,
+                (long long)(bytes[6] / unit), (long long)unit, move_max_row_units());
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.k_block = bytes[0];
+  p.k_token = bytes[1];
+  p.k_head = bytes[2];
+  p.v_block = bytes[3];
+  p.v_token = bytes[4];
+  p.v_head = bytes[5];
+  p.row_bytes = static_cast<int>(bytes[6]);
+  p.unit = static_cast<int>(unit);
+  p.num_blocks = num_blocks;
+  p.page_size = page_size;
+  p.page_div = FastDiv(static_cast<uint32_t>(page_size));
+  p.requests = requests;
+  p.kv_heads = num_kv_heads;
+  p.head_div = FastDiv(static_cast<uint32_t>(num_kv_heads));
+  p.table = block_table;
+  p.table_stride = table_stride;
+  p.table_width = table_width;
+  p.in_place = out_table == nullptr || out_table == block_table;
+  p.out_table = p.in_place ? block_table : out_table;
+  p.out_table_stride = p.in_place ? table_stride : out_table_stride;
+  p.out_table_width = p.in_place ? table_width : out_table_width;
+  p.err = device_error_word();
+  return QSA_OK;
+}
+
+int qsa_cache_compact(void* k_cache, int64_t k_block_stride, int64_t k_token_stride,
+                      int64_t k_head_stride, void* v_cache, int64_t v_block_stride,
+                      int64_t v_token_stride, int64_t v_head_stride, int64_t num_blocks,
+                      int32_t page_size, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                      const int32_t* block_table, int64_t table_row_stride, int32_t table_width,
+                      const int32_t* out_table, int64_t out_table_row_stride,
+                      int32_t out_table_width, int32_t num_requests, const int32_t* indices,
+                      int64_t indices_request_stride, int64_t indices_head_stride, int32_t count,
+                      const int32_t* starts, void* stream) {
+  const char* who = "qsa_cache_compact";
+  MoveParams p = {};
+  const int status = move_common(
+      p, who, k_cache, k_block_stride, k_token_stride, k_head_stride, v_cache, v_block_stride,
+      v_token_stride, v_head_stride, num_blocks, page_size, num_kv_heads, head_dim, dtype,
+      block_table, table_row_stride, table_width, out_table, out_table_row_stride, out_table_width,
+      num_requests);
+  if (status != QSA_OK) return status;
+  if (count < 0) return fail(QSA_ERR_INVALID, "%s: negative count", who);
+  if (count == 0 || num_requests == 0) return QSA_OK;
+  if (!indices) return fail(QSA_ERR_INVALID, "%s: null indices", who);
+  p.count = count;
+  p.indices = indices;
+  p.idx_req_stride = indices_request_stride;
+  p.idx_head_stride = indices_head_stride;
+  p.list_heads = num_kv_heads;
+  p.list_div = p.head_div;
+  p.starts = starts;
+  cudaError_t e = launch_cache_compact(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return QSA_OK;
+}
+
+static size_t evict_chosen_offset(int32_t requests, int32_t list_heads) {
+  return (static_cast<size_t>(requests) * list_heads * sizeof(int32_t) + 255) / 256 * 256;
+}
+
+size_t qsa_cache_evict_workspace_bytes(int32_t num_requests, int32_t list_heads, int32_t budget,
+                                       int32_t sinks, int32_t recent) {
+  if (num_requests <= 0 || list_heads <= 0 || sinks < 0 || recent < 0 ||
+      static_cast<int64_t>(budget) < static_cast<int64_t>(sinks) + recent)
+    return 0;  // no launch for these shapes
+  return evict_chosen_offset(num_requests, list_heads) +
+         static_cast<size_t>(num_requests) * list_heads * (budget - sinks - recent) *
+             sizeof(int32_t);
+}
+
+int qsa_cache_evict(const float* weights, int64_t weights_request_stride,
+                    int64_t weights_head_stride, int32_t list_heads, int32_t capacity,
+                    const int32_t* seq_lens, int32_t num_requests, int32_t budget, int32_t sinks,
+                    int32_t recent, void* k_cache, int64_t k_block_stride, int64_t k_token_stride,
+                    int64_t k_head_stride, void* v_cache, int64_t v_block_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, int64_t num_blocks,
+                    int32_t page_size, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                    const int32_t* block_table, int64_t table_row_stride, int32_t table_width,
+                    const int32_t* out_table, int64_t out_table_row_stride,
+                    int32_t out_table_width, float* weights_out, int64_t weights_out_request_stride,
+                    int64_t weights_out_head_stride, int32_t* kept, int32_t* lengths_out,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "qsa_cache_evict";
+  MoveParams p = {};
+  const int status = move_common(
+      p, who, k_cache, k_block_stride, k_token_stride, k_head_stride, v_cache, v_block_stride,
+      v_token_stride, v_head_stride, num_blocks, page_size, num_kv_heads, head_dim, dtype,
+      block_table, table_row_stride, table_width, out_table, out_table_row_stride, out_table_width,
+      num_requests);
+  if (status != QSA_OK) return status;
+  if (list_heads != 1 && list_heads != num_kv_heads)
+    return fail(QSA_ERR_INVALID, "%s: weights of %d heads (1 or %d expected)", who, list_heads,
+                num_kv_heads);
+  if (capacity < 0 || budget < 0 || sinks < 0 || recent < 0 ||
+      static_cast<int64_t>(sinks) + recent > budget)
+    return fail(QSA_ERR_INVALID, "%s: sinks %d + recent %d must fit the budget %d", who, sinks,
+                recent, budget);
+  if (num_requests == 0) return QSA_OK;
+  if ((capacity > 0 && (!weights || !weights_out)) || !seq_lens || (budget > 0 && !kept) ||
+      !lengths_out)
+    return fail(QSA_ERR_INVALID, "%s: null pointer", who);
+  if (list_heads > 1 && num_requests > 1 &&
+      weights_request_stride != weights_head_stride * list_heads)
+    return fail(QSA_ERR_INVALID, "%s: weights' (request, head) rows must be evenly spaced", who);
+  const int64_t row_stride = list_heads > 1 ? weights_head_stride : weights_request_stride;
+  const int chosen = budget - sinks - recent;
+  if (capacity > budget && chosen > 0) {
+    if (capacity - sinks - recent > topk_max_width())
+      return fail(QSA_ERR_UNSUPPORTED, "%s: %d tokens to choose from exceed %d", who,
+                  capacity - sinks - recent, topk_max_width());
+    if (chosen > topk_max_blocks())
+      return fail(QSA_ERR_UNSUPPORTED, "%s: %d tokens to choose exceed %d", who, chosen,
+                  topk_max_blocks());
+    if ((num_requests > 1 || list_heads > 1) && row_stride < capacity)
+      return fail(QSA_ERR_INVALID, "%s: weights row stride %lld < %d", who, (long long)row_stride,
+                  capacity);
+  }
+  const size_t need =
+      qsa_cache_evict_workspace_bytes(num_requests, list_heads, budget, sinks, recent);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(QSA_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu required", who, workspace_bytes,
+                need);
+  if (!aligned(workspace, 256))
+    return fail(QSA_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
+  p.count = budget;
+  p.list_heads = list_heads;
+  p.list_div = FastDiv(static_cast<uint32_t>(list_heads));
+  p.evict = 1;
+  p.budget = budget;
+  p.sinks = sinks;
+  p.recent = recent;
+  p.capacity = capacity;
+  p.seq_lens = seq_lens;
+  int32_t* middle = static_cast<int32_t*>(workspace);
+  int32_t* list = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) +
+                                             evict_chosen_offset(num_requests, list_heads));
+  p.chosen = list;
+  p.chosen_width = chosen;
+  p.weights = weights;
+  p.w_req_stride = weights_request_stride;
+  p.w_head_stride = weights_head_stride;
+  p.weights_out = weights_out;
+  p.wo_req_stride = weights_out_request_stride;
+  p.wo_head_stride = weights_out_head_stride;
+  p.kept = kept;
+  cudaError_t e = launch_cache_evict(p, lengths_out, middle, list,
+                                     static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return QSA_OK;
+}
+
 // -------------------------------------------------------------- attention
 size_t qsa_sparse_attention_workspace_bytes(int32_t rows, int32_t num_q_heads,
                                             int32_t num_kv_heads, int32_t head_dim,

@@ -251,6 +251,49 @@ struct RotaryParams {
 };
 cudaError_t launch_rotary(RotaryParams p, cudaStream_t stream);
 
+// ------------------------------------------------------------ cache moves
+struct MoveParams {
+  void *k_cache, *v_cache;
+  int64_t k_block, k_token, k_head, v_block, v_token, v_head;  // strides in BYTES
+  int64_t num_blocks;
+  int page_size;
+  FastDiv page_div;
+  int requests, kv_heads;
+  FastDiv head_div;        // division by kv_heads
+  const int32_t *table, *out_table;
+  int64_t table_stride, out_table_stride;
+  int table_width, out_table_width;
+  int in_place;            // out_table is table
+  int row_bytes;           // bytes of one head's key (or value) row
+  int unit;                // bytes of one copy: 16, 4 or 2
+  int count;               // entries of each list
+  int list_heads;          // kv_heads, or 1 for a list shared by all heads
+  FastDiv list_div;        // division by list_heads
+  const int32_t* starts;   // first destination token of each request; nullptr: 0
+  // compaction: the lists
+  const int32_t* indices;
+  int64_t idx_req_stride, idx_head_stride;
+  // eviction (count == budget)
+  int evict, budget, sinks, recent, capacity;
+  const int32_t* seq_lens;
+  const int32_t* chosen;   // [requests, list_heads, chosen_width], relative to `sinks`
+  int chosen_width;        // budget - sinks - recent
+  const float* weights;
+  int64_t w_req_stride, w_head_stride;
+  float* weights_out;
+  int64_t wo_req_stride, wo_head_stride;
+  int32_t* kept;           // [requests, list_heads, budget] or nullptr
+  int* err;
+  // filled by the launcher
+  int row_units, group;
+  FastDiv lane_div;
+};
+// Most copy units of one row that a block takes.
+int move_max_row_units();
+cudaError_t launch_cache_compact(const MoveParams& p, cudaStream_t stream);
+cudaError_t launch_cache_evict(const MoveParams& p, int32_t* lengths_out, int32_t* middle,
+                               int32_t* chosen, cudaStream_t stream);
+
 int num_sms();
 // One CTA waits on an mbarrier phase nothing completes; the bounded wait
 // expires and records kDeviceErrWaitTimeout in *err (selftest.cu).

@@ -1,0 +1,203 @@
+"""Compaction and eviction of cached tokens: exact, against a plain restatement on the host."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch.device("cuda")
+
+
+def pool(g, dev, requests, ctx, page, hkv, d, dtype, more=0, fused=True, shift=0):
+    width = -(-ctx // page) if ctx else 1
+    blocks = requests * (width + more) + 2
+    if fused:
+        buf = torch.randn(blocks, page, hkv, 2 * d + shift, generator=g).to(dtype).to(dev)
+        k, v = buf[..., shift:d + shift], buf[..., d + shift:]
+    else:
+        buf = torch.randn(2, blocks, hkv, page, d, generator=g).to(dtype).to(dev)
+        k, v = buf[0].transpose(1, 2), buf[1].transpose(1, 2)
+    pages = torch.randperm(blocks, generator=g)[: requests * (width + more)].to(torch.int32)
+    return (k, v, pages[: requests * width].view(requests, width).to(dev),
+            pages[requests * width:].view(requests, more).to(dev))
+
+
+def moved(k, v, table, out_table, lists, starts):
+    """The caches after the moves; lists[b][h]: the sources."""
+    k0, v0, page = k.cpu(), v.cpu(), k.shape[1]
+    k1, v1 = k0.clone(), v0.clone()
+    table, out_table = table.cpu().long(), out_table.cpu().long()
+    for b, heads in enumerate(lists):
+        for h, sources in enumerate(heads):
+            for j, s in enumerate(sources):
+                if s < 0:
+                    continue
+                t = starts[b] + j
+                a, at = table[b, s // page], s % page
+                o, ot = out_table[b, t // page], t % page
+                k1[o, ot, h], v1[o, ot, h] = k0[a, at, h], v0[a, at, h]
+    return k1, v1
+
+
+CASES = [  # requests, ctx, page, heads, d, dtype, count, start, per head, fused, shift
+    (1, 1, 16, 1, 64, BF16, 1, 0, False, True, 0),
+    (3, 200, 16, 2, 128, BF16, 37, 11, True, True, 0),
+    (5, 333, 1, 4, 64, F16, 300, 0, False, False, 0),
+    (2, 2500, 64, 8, 128, BF16, 1900, 100, True, True, 0),
+    (1, 9000, 48, 1, 128, F32, 8000, 5, True, True, 0),
+    (2, 700, 20, 3, 40, BF16, 600, 50, False, True, 4),   # rows at odd offsets: 8-byte aligned
+    (2, 300, 16, 2, 31, F16, 250, 7, True, True, 1),       # rows of an odd length: 2-byte copies
+    (40, 257, 32, 8, 256, BF16, 100, 1, True, True, 0),
+    (2, 600, 16, 1, 2048, BF16, 100, 3, False, True, 0),
+]
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("requests,ctx,page,hkv,d,dtype,count,start,per_head,fused,shift", CASES)
+def test_compact(dev, in_place, requests, ctx, page, hkv, d, dtype, count, start, per_head, fused,
+                 shift):
+    from qsa_vllm_b200 import _lib
+    from qsa_vllm_b200.eviction import cache_compact
+    g = torch.Generator().manual_seed(ctx + count)
+    k, v, table, other = pool(g, dev, requests, ctx, page, hkv, d, dtype,
+                              0 if in_place else -(-ctx // page), fused, shift)
+    heads = hkv if per_head else 1
+    idx = torch.rand(requests, heads, ctx - start, generator=g).argsort(-1)[..., :count]
+    idx = (idx.sort(-1).values + start).to(torch.int32)
+    idx[torch.rand(idx.shape, generator=g) < 0.1] = -1
+    starts = torch.full((requests,), start, dtype=torch.int32)
+    lists = idx.expand(-1, hkv, -1).tolist()
+    want = moved(k, v, table, table if in_place else other, lists, starts.tolist())
+    arg = idx.to(dev) if per_head else idx[:, 0].contiguous().to(dev)
+    cache_compact(k, v, table, arg, starts.to(dev), out_table=None if in_place else other)
+    assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+    assert _lib.device_error_poll() == 0
+
+
+def test_compact_in_place_many_times_over_itself(dev):
+    """Dense lists of long contexts: each destination is another row's source, several groups
+    and several clusters' rounds apart."""
+    from qsa_vllm_b200.eviction import cache_compact
+    g = torch.Generator().manual_seed(1)
+    k, v, table, _ = pool(g, dev, 2, 20000, 16, 2, 64, BF16)
+    for drop in (1, 2, 700):
+        idx = torch.stack([torch.cat([torch.arange(3), torch.arange(3 + drop + b, 19000 + b)])[:18000]
+                           for b in range(2)]).to(torch.int32)
+        want = moved(k, v, table, table, [[r] * 2 for r in idx.tolist()], [0, 0])
+        cache_compact(k, v, table, idx.to(dev))
+        assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+
+
+def test_compact_skips_and_reports_what_it_cannot_move(dev):
+    from qsa_vllm_b200 import _lib
+    from qsa_vllm_b200.eviction import cache_compact
+    g = torch.Generator().manual_seed(2)
+    k, v, table, _ = pool(g, dev, 1, 64, 16, 1, 64, BF16)
+    table[0, 2] = -1
+    for idx, start in ([40], 0), ([64], 0), ([2**31 - 1], 0), ([3], 5), ([5], 40), ([5], -1):
+        k0, v0 = k.clone(), v.clone()
+        cache_compact(k, v, table, torch.tensor([idx], dtype=torch.int32, device=dev),
+                      torch.tensor([start], dtype=torch.int32, device=dev))
+        assert _lib.device_error_poll() == 2, (idx, start)
+        assert torch.equal(k, k0) and torch.equal(v, v0)
+    cache_compact(k, v, table, torch.empty(1, 0, dtype=torch.int32, device=dev))
+    cache_compact(k, v, table[:0], torch.empty(0, 4, dtype=torch.int32, device=dev))
+    assert torch.equal(k, k0) and _lib.device_error_poll() == 0
+
+
+def chosen(w, n, budget, sinks, recent):
+    if n <= budget:
+        return list(range(n))
+    middle = w[sinks:n - recent].double()
+    best = (-middle).sort(stable=True).indices[: budget - sinks - recent].sort().values + sinks
+    return list(range(sinks)) + best.tolist() + list(range(n - recent, n))
+
+
+EVICT = [  # lengths, capacity, budget, sinks, recent, page, heads, d, dtype, shared
+    ([0, 1, 5, 9, 17], 17, 9, 2, 3, 16, 2, 64, BF16, False),
+    ([100, 257, 64, 65], 257, 64, 4, 16, 16, 4, 128, BF16, False),
+    ([300] * 3, 300, 299, 0, 0, 32, 1, 64, F16, False),
+    ([777, 2], 1000, 100, 100, 0, 8, 2, 128, BF16, False),   # nothing left to choose
+    ([777, 500], 800, 100, 0, 100, 8, 2, 128, BF16, True),
+    ([5000, 3000, 5001], 5003, 1201, 4, 128, 64, 2, 128, BF16, True),
+    ([40000], 40000, 5000, 16, 1024, 64, 1, 64, F32, False),
+    ([2112, 2049, 2048], 2112, 2048, 4, 512, 16, 8, 128, BF16, False),
+    ([50, 60], 60, 0, 0, 0, 16, 2, 64, BF16, False),          # a budget of nothing
+    ([70, 300], 64, 32, 1, 1, 16, 2, 64, BF16, False),        # lengths past the capacity
+    ([70, 300], 0, 8, 1, 1, 16, 2, 64, BF16, False),          # a capacity of nothing
+]
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("lengths,capacity,budget,sinks,recent,page,hkv,d,dtype,shared", EVICT)
+def test_evict(dev, in_place, lengths, capacity, budget, sinks, recent, page, hkv, d, dtype,
+               shared):
+    from qsa_vllm_b200 import _lib
+    from qsa_vllm_b200.eviction import cache_evict
+    g = torch.Generator().manual_seed(capacity + budget)
+    requests, heads = len(lengths), 1 if shared else hkv
+    k, v, table, other = pool(g, dev, requests, max(capacity, *lengths), page, hkv, d, dtype,
+                              0 if in_place else -(-max(budget, capacity) // page))
+    # weights with many ties, at zero and elsewhere
+    w = torch.randint(0, 40, (requests, heads, capacity + 3), generator=g).float()
+    w = torch.where(torch.rand(w.shape, generator=g) < 0.3, w * torch.rand(w.shape, generator=g), w)
+    w = w.to(dev)[..., :capacity]
+    counted = [min(n, capacity) for n in lengths]
+    keep = [[chosen(w[b, h].cpu(), n, budget, sinks, recent) for h in range(heads)]
+            for b, n in enumerate(counted)]
+    lists = [r * hkv if shared else r for r in keep]
+    want = moved(k, v, table, table if in_place else other, lists, [0] * requests)
+    w_out = None if in_place else torch.full((requests, heads, capacity), -5.0, device=dev)
+    w_want = (w.clone() if in_place else w_out.clone()).cpu()
+    for b, n in enumerate(counted):
+        for h in range(heads):
+            at = keep[b][h]
+            w_want[b, h, :len(at)] = w[b, h].cpu()[at]
+            w_want[b, h, len(at):n] = 0
+    seq = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    kept, count = cache_evict(w, seq, table, k, v, budget, sinks=sinks, recent=recent,
+                              out_table=None if in_place else other, weights_out=w_out)
+    assert count.tolist() == [min(n, budget) for n in counted]
+    assert seq.tolist() == lengths
+    for b in range(requests):
+        for h in range(heads):
+            n = len(keep[b][h])
+            assert kept[b, h, :n].tolist() == keep[b][h] and (kept[b, h, n:] == -1).all()
+    assert torch.equal((w if in_place else w_out).cpu(), w_want)
+    assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+    assert _lib.device_error_poll() == 0
+
+
+def test_evict_captured_again_and_again(dev):
+    """A captured step that grows and evicts: the lengths are the device's, not the capture's."""
+    from qsa_vllm_b200.eviction import cache_evict
+    g = torch.Generator().manual_seed(8)
+    k, v, table, _ = pool(g, dev, 2, 128, 16, 2, 64, BF16)
+    w = torch.rand(2, 2, 128, generator=g).to(dev)
+    seq = torch.tensor([100, 90], dtype=torch.int32, device=dev)
+    start = [t.clone() for t in (k, v, w, seq)]
+
+    def step():
+        _, count = cache_evict(w, seq, table, k, v, 64, sinks=2, recent=8)
+        seq.copy_(count + 30)
+
+    for _ in range(3):
+        step()
+    want = [t.clone() for t in (k, v, w, seq)]
+    for t, s in zip((k, v, w, seq), start):
+        t.copy_(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for t, s in zip((k, v, w, seq), want):
+        assert torch.equal(t, s)

@@ -87,3 +87,82 @@ def test_rotary_c_abi_refusals():
             (dict(pos=None), 1, b"null"), (dict(hkv=1), 1, b"null"), (dict(q=4097), 1, b"aligned"),
             (dict(hq=70000), 2, b"heads")):
         assert call(**bad) == status and word in lib.qsa_last_error(), bad
+
+
+def _cache(requests=2, page=16, hkv=2, d=64, dtype=BF16):
+    kv = torch.zeros(8, page, hkv, 2 * d, dtype=dtype)
+    return kv[..., :d], kv[..., d:], torch.zeros(requests, 4, dtype=torch.int32)
+
+
+def test_compact_refusals():
+    from qsa_vllm_b200 import QSAError
+    from qsa_vllm_b200.eviction import cache_compact
+    k, v, table = _cache()
+    idx = torch.zeros(2, 3, dtype=torch.int32)
+    for args, err in (((k[0], v[0], table, idx), ValueError), ((k, v.float(), table, idx), TypeError),
+                      ((k, v, table.long(), idx), TypeError), ((k, v, table, idx.long()), TypeError),
+                      ((k, v, table, idx[:1]), ValueError),
+                      ((k, v, table, idx[:, None].expand(2, 3, 3)), ValueError),
+                      ((k, v, table, idx.t().contiguous().t()), ValueError),
+                      ((k, v, table, idx, idx[:, 0].long()), TypeError),
+                      ((k, v, table, idx, torch.zeros(3, dtype=torch.int32)), ValueError),
+                      ((k.double(), v.double(), table, idx), TypeError)):
+        with pytest.raises(err):
+            cache_compact(*args)
+    with pytest.raises(ValueError, match="out_table"):
+        cache_compact(k, v, table, idx, out_table=table[:1])
+    with pytest.raises(QSAError):
+        cache_compact(k, v, table, idx)
+
+
+def test_evict_refusals():
+    from qsa_vllm_b200 import QSAError
+    from qsa_vllm_b200.eviction import cache_evict, cache_evict_workspace_bytes
+    k, v, table = _cache()
+    w, seq = torch.zeros(2, 2, 64), torch.zeros(2, dtype=torch.int32)
+
+    def call(err, w=w, seq=seq, budget=16, match=None, **more):
+        with pytest.raises(err, match=match):
+            cache_evict(w, seq, table, k, v, budget, **more)
+    call(TypeError, w=w.double())
+    call(ValueError, w=w[0])
+    call(ValueError, w=torch.zeros(2, 3, 64))
+    call(ValueError, w=w.transpose(1, 2).contiguous().transpose(1, 2))
+    call(ValueError, weights_out=torch.zeros(2, 2, 63))
+    call(TypeError, seq=seq.long())
+    call(ValueError, seq=seq[:1])
+    call(ValueError, sinks=10, recent=7)
+    call(ValueError, sinks=-1)
+    call(ValueError, kept=torch.zeros(2, 2, 15, dtype=torch.int32))
+    call(QSAError)
+    assert cache_evict_workspace_bytes(0, 2, 16, 0, 0) == 0
+    assert cache_evict_workspace_bytes(2, 2, 16, 10, 7) == 0
+    assert cache_evict_workspace_bytes(2, 2, 16, 2, 4) == 256 + 2 * 2 * 10 * 4
+
+
+def test_cache_move_c_abi_refusals():
+    from qsa_vllm_b200 import _lib
+    lib = _lib.load_library()
+
+    def compact(k=4096, page=16, heads=2, dim=64, dtype=0, requests=2, idx=4096, n=3, table=4096):
+        return lib.qsa_cache_compact(k, 1, 1, 64, 4096, 64, 64, 64, 8, page, heads, dim, dtype,
+                                     table, 4, 4, None, 0, 0, requests, idx, 3, 0, n, None, None)
+    assert compact(requests=0) == 0 and compact(n=0) == 0
+    for bad, status, word in (
+            (dict(k=None), 1, b"null"), (dict(idx=None), 1, b"null"), (dict(table=None), 1, b"null"),
+            (dict(page=0), 1, b"sizes"), (dict(heads=0), 1, b"sizes"), (dict(dim=-1), 1, b"sizes"),
+            (dict(dtype=7), 1, b"dtype"), (dict(n=-1), 1, b"count"), (dict(k=4097), 1, b"aligned"),
+            (dict(requests=65536), 2, b"65535"), (dict(dim=4096), 2, b"units")):
+        assert compact(**bad) == status and word in lib.qsa_last_error(), bad
+
+    def evict(w=4096, heads=2, cap=64, budget=16, sinks=2, recent=4, stride=128, ws=4096, n=1 << 20):
+        return lib.qsa_cache_evict(w, stride, 64, heads, cap, 4096, 2, budget, sinks, recent, 4096,
+                                   64, 64, 64, 4096, 64, 64, 64, 8, 16, 2, 64, 0, 4096, 4, 4, None,
+                                   0, 0, 4096, 128, 64, 4096, 4096, ws, n, None)
+    for bad, status, word in (
+            (dict(w=None), 1, b"null"), (dict(heads=3), 1, b"heads"), (dict(budget=5), 1, b"budget"),
+            (dict(budget=-1), 1, b"budget"), (dict(stride=100), 1, b"evenly"),
+            (dict(cap=1 << 20, heads=1, stride=1 << 20), 2, b"choose"),
+            (dict(ws=None), 3, b"workspace"), (dict(n=100), 3, b"workspace"),
+            (dict(ws=4100), 1, b"aligned"), (dict(cap=65, heads=1, stride=64), 1, b"stride")):
+        assert evict(**bad) == status and word in lib.qsa_last_error(), bad
