@@ -411,6 +411,76 @@ QSA_API int qsa_rotary(
     const double* frequencies, int32_t rotary_dim, float factor, int32_t interleaved,
     int32_t inverse, int32_t dtype, void* stream);
 
+/* Workspace bytes of qsa_tree_attention (0 for shapes it rejects). */
+QSA_API size_t qsa_tree_attention_workspace_bytes(int32_t rows, int32_t num_requests,
+                                                  int32_t num_q_heads, int32_t num_kv_heads,
+                                                  int32_t head_dim, int32_t max_query_len);
+
+/*
+ * Attention of drafted-token trees over the paged cache.  No counterpart in
+ * the reference, whose decode rows each attend a selection.
+ *
+ * Request b owns the packed rows query_start_loc[b] .. query_start_loc[b+1]-1
+ * (int32 [num_requests + 1], non-decreasing): its drafted tokens, whose keys
+ * and values are already cached as the last ones of its seq_lens[b] tokens.
+ * Every row sees all tokens before those; row i sees drafted token j when
+ * tree_mask[row, j] != 0 (uint8 [rows, mask_width], columns past mask_width
+ * unseen), or, with tree_mask NULL, when j <= i (a chain: a decode step or a
+ * causal prompt chunk).  For query head h and kv head h / (num_q_heads /
+ * num_kv_heads):
+ *   out[row,h] = sum_t p_t v_t,  p = softmax over the seen t of scale * q.k_t
+ *   lse[row,h] = log sum_t exp(scale * q.k_t)    (fp32, natural, nullable)
+ * A row that sees nothing gets out 0 and lse -inf.  Tokens past the block
+ * table or on unmapped pages (below 0 or past num_blocks) are not seen.  Keys
+ * and values of tokens past seq_lens, and of drafted tokens that a row does
+ * not see, may hold anything.  Rows of no request are not written.
+ * Sums, maxima and lse are fp32; p is rounded to the tensors' type before the
+ * product with v, the output once.
+ * q, out: [rows, num_q_heads, head_dim]; k_cache, v_cache: [num_blocks,
+ * page_size, num_kv_heads, head_dim]; bf16 or fp16, unit dim strides, 16-byte
+ * aligned rows of q and caches.  head_dim a multiple of 8 up to 256; head_dim
+ * 64 / 128 with pages that are a multiple of 8 run on the tensor cores.
+ * max_query_len sizes the work split (the longest request's rows; a smaller
+ * value costs speed, not results).
+ */
+QSA_API int qsa_tree_attention(
+    const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t rows, int32_t num_q_heads,
+    int32_t head_dim, int32_t dtype, const void* k_cache, int64_t k_block_stride,
+    int64_t k_token_stride, int64_t k_head_stride, const void* v_cache, int64_t v_block_stride,
+    int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks, int32_t page_size,
+    int32_t num_kv_heads, const int32_t* block_table, int64_t table_row_stride,
+    int32_t table_width, int32_t num_requests, const int32_t* seq_lens,
+    const int32_t* query_start_loc, const uint8_t* tree_mask, int64_t mask_row_stride,
+    int32_t mask_width, int32_t max_query_len, float scale, void* out, int64_t out_row_stride,
+    int64_t out_head_stride, float* lse, int64_t lse_row_stride, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/*
+ * Attention weight that each cached token has received.  No counterpart in
+ * the reference.
+ *   weights_out[b, kv, t] = weights[b, kv, t] +
+ *       sum over b's rows i of row_factors[i] * sum over the query heads h of
+ *       kv of exp(scale * q[i,h].k_t - lse[i,h])        for the rows that see t
+ * for t < min(seq_lens[b], capacity, table_width * page_size); others are not
+ * written.  lse as qsa_tree_attention leaves it, the other arguments as there.
+ * row_factors (fp32 [rows], NULL: 1) picks the rows that count, 0 for rejected
+ * drafts; rows with factor 0 or lse -inf add nothing.  weights, weights_out:
+ * fp32 [num_requests, num_kv_heads, capacity], unit token stride, the same
+ * buffer or apart.  Sums are fp32 in a fixed order (no atomics).
+ */
+QSA_API int qsa_attention_weights(
+    const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t rows, int32_t num_q_heads,
+    int32_t head_dim, int32_t dtype, const void* k_cache, int64_t k_block_stride,
+    int64_t k_token_stride, int64_t k_head_stride, int32_t num_blocks, int32_t page_size,
+    int32_t num_kv_heads, const int32_t* block_table, int64_t table_row_stride,
+    int32_t table_width, int32_t num_requests, const int32_t* seq_lens,
+    const int32_t* query_start_loc, const uint8_t* tree_mask, int64_t mask_row_stride,
+    int32_t mask_width, int32_t max_query_len, float scale, const float* lse,
+    int64_t lse_row_stride, const float* row_factors, int64_t row_factors_stride,
+    const float* weights, int64_t weights_request_stride, int64_t weights_head_stride,
+    float* weights_out, int64_t weights_out_request_stride, int64_t weights_out_head_stride,
+    int32_t capacity, void* stream);
+
 /*
  * Compaction of cached tokens.  No counterpart in the reference.
  *

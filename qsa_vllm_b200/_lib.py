@@ -62,6 +62,15 @@ SIGNATURES: dict[str, tuple] = {
         _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64,
         _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64,
         _i32, _i32, _vp, _i64, C.c_void_p, _i32, _f32, _i32, _i32, _i32, _vp]),
+    "qsa_tree_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "qsa_tree_attention": (C.c_int, [
+        _vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64,
+        _i32, _i32, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _f32,
+        _vp, _i64, _i64, _vp, _i64, _vp, _sz, _vp]),
+    "qsa_attention_weights": (C.c_int, [
+        _vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _i64,
+        _i32, _i32, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _f32,
+        _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp]),
     "qsa_cache_compact": (C.c_int, [
         _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
         _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _i32, _vp, _vp]),

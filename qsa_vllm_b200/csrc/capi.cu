@@ -912,6 +912,176 @@ int qsa_cache_evict(const float* weights, int64_t weights_request_stride,
   return QSA_OK;
 }
 
+// --------------------------------------- attention of drafted-token trees
+// What qsa_tree_attention and qsa_attention_weights share; the value cache is
+// null for the latter.
+static int tree_common(TreeParams& p, const char* who, const void* q, int64_t q_row_stride,
+                       int64_t q_head_stride, int32_t rows, int32_t num_q_heads, int32_t head_dim,
+                       int32_t dtype, const void* k_cache, int64_t k_block_stride,
+                       int64_t k_token_stride, int64_t k_head_stride, int32_t num_blocks,
+                       int32_t page_size, int32_t num_kv_heads, const int32_t* block_table,
+                       int64_t table_row_stride, int32_t table_width, int32_t num_requests,
+                       const int32_t* seq_lens, const int32_t* query_start_loc,
+                       const uint8_t* tree_mask, int64_t mask_row_stride, int32_t mask_width,
+                       int32_t max_query_len, float scale) {
+  if (rows < 0 || num_requests < 0 || mask_width < 0)
+    return fail(QSA_ERR_INVALID, "%s: negative size", who);
+  if (dtype != QSA_DTYPE_BF16 && dtype != QSA_DTYPE_F16)
+    return fail(QSA_ERR_UNSUPPORTED, "%s: dtype %d (bf16 and fp16 supported)", who, dtype);
+  if (head_dim <= 0 || head_dim % 8 || head_dim > 256)
+    return fail(QSA_ERR_UNSUPPORTED, "%s: head_dim %d (multiples of 8 up to 256 supported)", who,
+                head_dim);
+  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
+    return fail(QSA_ERR_INVALID, "%s: %d query heads not a multiple of %d kv heads", who,
+                num_q_heads, num_kv_heads);
+  if (num_kv_heads > 65535 || static_cast<int64_t>(num_requests) * num_kv_heads > 65535)
+    return fail(QSA_ERR_UNSUPPORTED, "%s: %d requests x %d heads exceed 65535", who, num_requests,
+                num_kv_heads);
+  if (page_size <= 0 || num_blocks < 0 || table_width < 0)
+    return fail(QSA_ERR_INVALID, "%s: bad page geometry", who);
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(QSA_ERR_INVALID, "%s: scale must be positive and finite", who);
+  if (num_requests == 0) return QSA_OK;
+  if (max_query_len <= 0) return fail(QSA_ERR_INVALID, "%s: max_query_len must be positive", who);
+  if ((rows > 0 && !q) || !k_cache || !block_table || !seq_lens || !query_start_loc)
+    return fail(QSA_ERR_INVALID, "%s: null pointer", who);
+  if (!aligned(k_cache, 16) || k_block_stride % 8 || k_token_stride % 8 || k_head_stride % 8)
+    return fail(QSA_ERR_INVALID, "%s: cache rows must be 16-byte aligned", who);
+  if (!aligned(q, 16) || q_row_stride % 8 || q_head_stride % 8)
+    return fail(QSA_ERR_INVALID, "%s: q head rows must be 16-byte aligned", who);
+  p.q = q;
+  p.q_row_stride = q_row_stride;
+  p.q_head_stride = q_head_stride;
+  p.rows = rows;
+  p.q_heads = num_q_heads;
+  p.kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
+  p.dim = head_dim;
+  p.dtype = dtype;
+  p.k_cache = k_cache;
+  p.k_block_stride = k_block_stride;
+  p.k_token_stride = k_token_stride;
+  p.k_head_stride = k_head_stride;
+  p.num_blocks = num_blocks;
+  p.page_size = page_size;
+  p.page_div = FastDiv(static_cast<uint32_t>(page_size));
+  p.table = block_table;
+  p.table_stride = table_row_stride;
+  p.table_width = table_width;
+  p.requests = num_requests;
+  p.seq_lens = seq_lens;
+  p.query_start_loc = query_start_loc;
+  p.mask = tree_mask;
+  p.mask_stride = mask_row_stride;
+  p.mask_width = mask_width;
+  p.scale = scale;
+  p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  p.max_query_len = max_query_len;
+  p.err = device_error_word();
+  return QSA_OK;
+}
+
+size_t qsa_tree_attention_workspace_bytes(int32_t rows, int32_t num_requests, int32_t num_q_heads,
+                                          int32_t num_kv_heads, int32_t head_dim,
+                                          int32_t max_query_len) {
+  if (rows <= 0 || num_requests <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
+      num_q_heads % num_kv_heads || max_query_len <= 0)
+    return 0;  // no launch for these shapes
+  return tree_attention_workspace(rows, num_requests, num_q_heads, num_kv_heads, head_dim,
+                                  max_query_len);
+}
+
+int qsa_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t rows,
+                       int32_t num_q_heads, int32_t head_dim, int32_t dtype, const void* k_cache,
+                       int64_t k_block_stride, int64_t k_token_stride, int64_t k_head_stride,
+                       const void* v_cache, int64_t v_block_stride, int64_t v_token_stride,
+                       int64_t v_head_stride, int32_t num_blocks, int32_t page_size,
+                       int32_t num_kv_heads, const int32_t* block_table, int64_t table_row_stride,
+                       int32_t table_width, int32_t num_requests, const int32_t* seq_lens,
+                       const int32_t* query_start_loc, const uint8_t* tree_mask,
+                       int64_t mask_row_stride, int32_t mask_width, int32_t max_query_len,
+                       float scale, void* out, int64_t out_row_stride, int64_t out_head_stride,
+                       float* lse, int64_t lse_row_stride, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  const char* who = "qsa_tree_attention";
+  TreeParams p = {};
+  const int status = tree_common(p, who, q, q_row_stride, q_head_stride, rows, num_q_heads,
+                                 head_dim, dtype, k_cache, k_block_stride, k_token_stride,
+                                 k_head_stride, num_blocks, page_size, num_kv_heads, block_table,
+                                 table_row_stride, table_width, num_requests, seq_lens,
+                                 query_start_loc, tree_mask, mask_row_stride, mask_width,
+                                 max_query_len, scale);
+  if (status != QSA_OK) return status;
+  if (rows == 0 || num_requests == 0) return QSA_OK;
+  if (!v_cache || !out) return fail(QSA_ERR_INVALID, "%s: null pointer", who);
+  if (!aligned(v_cache, 16) || v_block_stride % 8 || v_token_stride % 8 || v_head_stride % 8)
+    return fail(QSA_ERR_INVALID, "%s: cache rows must be 16-byte aligned", who);
+  if (!aligned(out, 2)) return fail(QSA_ERR_INVALID, "%s: out must be 2-byte aligned", who);
+  const size_t need = tree_attention_workspace(rows, num_requests, num_q_heads, num_kv_heads,
+                                               head_dim, max_query_len);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(QSA_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu required", who, workspace_bytes,
+                need);
+  if (need > 0 && !aligned(workspace, 256))
+    return fail(QSA_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
+  p.v_cache = v_cache;
+  p.v_block_stride = v_block_stride;
+  p.v_token_stride = v_token_stride;
+  p.v_head_stride = v_head_stride;
+  p.out = out;
+  p.out_row_stride = out_row_stride;
+  p.out_head_stride = out_head_stride;
+  p.out_vec = aligned(out, 16) && out_row_stride % 8 == 0 && out_head_stride % 8 == 0;
+  p.lse = lse;
+  p.lse_row_stride = lse_row_stride;
+  p.workspace = workspace;
+  cudaError_t e = launch_tree_attention(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return QSA_OK;
+}
+
+int qsa_attention_weights(const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t rows,
+                          int32_t num_q_heads, int32_t head_dim, int32_t dtype,
+                          const void* k_cache, int64_t k_block_stride, int64_t k_token_stride,
+                          int64_t k_head_stride, int32_t num_blocks, int32_t page_size,
+                          int32_t num_kv_heads, const int32_t* block_table,
+                          int64_t table_row_stride, int32_t table_width, int32_t num_requests,
+                          const int32_t* seq_lens, const int32_t* query_start_loc,
+                          const uint8_t* tree_mask, int64_t mask_row_stride, int32_t mask_width,
+                          int32_t max_query_len, float scale, const float* lse,
+                          int64_t lse_row_stride, const float* row_factors,
+                          int64_t row_factors_stride, const float* weights,
+                          int64_t weights_request_stride, int64_t weights_head_stride,
+                          float* weights_out, int64_t weights_out_request_stride,
+                          int64_t weights_out_head_stride, int32_t capacity, void* stream) {
+  const char* who = "qsa_attention_weights";
+  TreeParams p = {};
+  const int status = tree_common(p, who, q, q_row_stride, q_head_stride, rows, num_q_heads,
+                                 head_dim, dtype, k_cache, k_block_stride, k_token_stride,
+                                 k_head_stride, num_blocks, page_size, num_kv_heads, block_table,
+                                 table_row_stride, table_width, num_requests, seq_lens,
+                                 query_start_loc, tree_mask, mask_row_stride, mask_width,
+                                 max_query_len, scale);
+  if (status != QSA_OK) return status;
+  if (capacity < 0) return fail(QSA_ERR_INVALID, "%s: negative capacity", who);
+  if (num_requests == 0 || capacity == 0) return QSA_OK;
+  if ((rows > 0 && !lse) || !weights || !weights_out) return fail(QSA_ERR_INVALID, "%s: null pointer", who);
+  p.lse = const_cast<float*>(lse);
+  p.lse_row_stride = lse_row_stride;
+  p.row_factors = row_factors;
+  p.factor_stride = row_factors_stride;
+  p.weights = weights;
+  p.w_req_stride = weights_request_stride;
+  p.w_head_stride = weights_head_stride;
+  p.weights_out = weights_out;
+  p.wo_req_stride = weights_out_request_stride;
+  p.wo_head_stride = weights_out_head_stride;
+  p.capacity = capacity;
+  cudaError_t e = launch_attention_weights(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return QSA_OK;
+}
+
 // -------------------------------------------------------------- attention
 size_t qsa_sparse_attention_workspace_bytes(int32_t rows, int32_t num_q_heads,
                                             int32_t num_kv_heads, int32_t head_dim,

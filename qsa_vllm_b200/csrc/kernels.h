@@ -294,6 +294,84 @@ cudaError_t launch_cache_compact(const MoveParams& p, cudaStream_t stream);
 cudaError_t launch_cache_evict(const MoveParams& p, int32_t* lengths_out, int32_t* middle,
                                int32_t* chosen, cudaStream_t stream);
 
+// --------------------------------------- attention of drafted-token trees
+struct TreeParams {
+  const void* q;           // [rows, q_heads, dim], unit dim stride
+  int64_t q_row_stride, q_head_stride;
+  int rows, q_heads, kv_heads, group, dim, dtype;
+  const void *k_cache, *v_cache;
+  int64_t k_block_stride, k_token_stride, k_head_stride;
+  int64_t v_block_stride, v_token_stride, v_head_stride;
+  int num_blocks, page_size;
+  FastDiv page_div;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_width, requests;
+  const int32_t *seq_lens, *query_start_loc;
+  const uint8_t* mask;     // [rows, mask_width]; nullptr: a chain
+  int64_t mask_stride;
+  int mask_width;
+  float scale, scale_log2;
+  int max_query_len;       // sizes the work split; not a limit
+  // attention
+  void* out;
+  int64_t out_row_stride, out_head_stride;
+  int out_vec;             // out rows 16-byte aligned
+  float* lse;              // nullable; attention weights: read
+  int64_t lse_row_stride;
+  // attention weights
+  const float* row_factors;  // nullable
+  int64_t factor_stride;
+  const float* weights;
+  int64_t w_req_stride, w_head_stride;
+  float* weights_out;
+  int64_t wo_req_stride, wo_head_stride;
+  int capacity;
+  void* workspace;
+  int* err;
+};
+
+// Request of packed row `row`, -1 if it belongs to none.
+__device__ __forceinline__ int tree_request(const TreeParams& p, int row) {
+  int lo = 0, hi = p.requests;  // first entry of query_start_loc[1..] above row
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.query_start_loc[mid + 1] > row) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo < p.requests && p.query_start_loc[lo] <= row ? lo : -1;
+}
+
+// What one request's rows see.  Its drafted tokens are the last `count` of
+// its `seq` cached ones: tokens below `prefix` are seen by every row, token
+// prefix + j by the rows whose mask says so (in a chain, by rows i >= j).
+struct TreeRequest {
+  int row0, count;  // packed rows
+  int prefix;       // may be negative
+  int tokens;       // cached tokens that the table reaches
+};
+__device__ __forceinline__ TreeRequest tree_request_info(const TreeParams& p, int b) {
+  TreeRequest r;
+  r.row0 = min(max(p.query_start_loc[b], 0), p.rows);
+  r.count = max(min(p.query_start_loc[b + 1], p.rows) - r.row0, 0);
+  const int seq = max(p.seq_lens[b], 0);
+  r.prefix = seq - r.count;
+  const int64_t reach = static_cast<int64_t>(p.table_width) * p.page_size;
+  r.tokens = static_cast<int>(reach < seq ? reach : seq);
+  return r;
+}
+// Whether packed row `row`, the request's row i, sees token t < r.tokens.
+__device__ __forceinline__ bool tree_sees(const TreeParams& p, const TreeRequest& r, int i, int t) {
+  const int node = t - r.prefix;
+  if (node < 0) return true;
+  if (p.mask == nullptr) return node <= i;
+  return node < p.mask_width && p.mask[(r.row0 + i) * p.mask_stride + node] != 0;
+}
+cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t stream);
+size_t tree_attention_workspace(int rows, int requests, int q_heads, int kv_heads, int dim,
+                                int max_query_len);
+cudaError_t launch_attention_weights(const TreeParams& p, cudaStream_t stream);
+
 int num_sms();
 // One CTA waits on an mbarrier phase nothing completes; the bounded wait
 // expires and records kDeviceErrWaitTimeout in *err (selftest.cu).

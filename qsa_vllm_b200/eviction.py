@@ -1,6 +1,8 @@
 """Keeping a paged cache small: the attention weight each cached token has received, the
 eviction that goes by it, and the compaction of cached tokens.
 
+* ``accumulate_attention_weights`` adds up, per KV head and cached token, the probabilities
+  that chosen rows gave it, from the log-sum-exp that ``tree_paged_attention`` left;
 * ``cache_evict`` keeps, per request and KV head, the first ``sinks`` tokens, the last
   ``recent`` ones and the heaviest of the rest, ``budget`` in all, and moves them to the front
   of the request's pages (or to other pages) in their order;
@@ -18,6 +20,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .qsa import aligned_head_rows
+from .tree_attention import check_tree_arguments, mask_arguments
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -53,6 +57,62 @@ def _cache_args(k_cache, v_cache, block_table, out_table) -> tuple:
             k_cache.shape[0], k_cache.shape[1], k_cache.shape[2], k_cache.shape[3],
             _DTYPES[k_cache.dtype], block_table.data_ptr(), block_table.stride(0),
             block_table.shape[1], *out)
+
+
+def accumulate_attention_weights(
+        q: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor,
+        seq_lens: torch.Tensor, query_start_loc: torch.Tensor, lse: torch.Tensor,
+        weights: torch.Tensor, out: torch.Tensor | None = None, *, max_query_len: int,
+        tree_mask: torch.Tensor | None = None, row_factors: torch.Tensor | None = None,
+        scale: float | None = None) -> torch.Tensor:
+    """``out[b, h, t] = weights[b, h, t] + sum_i row_factors[i] sum_g exp(scale q_ig.k_t -
+    lse_ig)`` over request b's rows i that see token t and the query heads g of KV head h.
+
+    Arguments as in ``tree_paged_attention``, whose ``lse`` this takes.  row_factors: fp32
+    ``[rows]``, 1 where None; 0 leaves a row out (a rejected draft).  weights, out: fp32 ``[B,
+    H_kv, capacity]``; out is weights itself (in place) where None.  Tokens from
+    ``min(seq_lens[b], capacity)`` on are not written."""
+    what = "accumulate_attention_weights"
+    max_query_len = int(max_query_len)
+    check_tree_arguments(what, q, (("k_cache", k_cache),), block_table, seq_lens,
+                         query_start_loc, tree_mask, max_query_len)
+    dev = q.device
+    rows, hq, d = q.shape
+    requests, hkv = block_table.shape[0], k_cache.shape[2]
+    if out is None:
+        out = weights
+    for name, w in (("weights", weights), ("out", out)):
+        if w.dtype != torch.float32 or w.device != dev:
+            raise TypeError(f"{what}: {name} must be float32 on {dev}")
+        if w.dim() != 3 or w.shape[:2] != (requests, hkv) or w.shape != weights.shape \
+                or (w.shape[2] > 1 and w.stride(2) != 1):
+            raise ValueError(f"{what}: {name} must be [{requests}, {hkv}, capacity] with a unit "
+                             "token stride")
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or lse.device != dev \
+            or (lse.stride(1) != 1 and hq > 1):
+        raise ValueError(f"{what}: lse must be float32 [rows, heads] with a unit head stride")
+    if row_factors is not None and (row_factors.dtype != torch.float32
+                                    or row_factors.shape != q.shape[:1]
+                                    or row_factors.device != dev):
+        raise ValueError(f"{what}: row_factors must be float32 [rows]")
+    _lib.ensure_device(dev)
+    if rows:
+        q = aligned_head_rows(q)
+    with _lib.on_device(dev):
+        _lib.check(_lib.load_library().qsa_attention_weights(
+            q.data_ptr(), q.stride(0), q.stride(1), rows, hq, d, _DTYPES[q.dtype],
+            k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+            k_cache.shape[0], k_cache.shape[1], hkv,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], requests,
+            seq_lens.data_ptr(), query_start_loc.data_ptr(),
+            *mask_arguments(tree_mask, seq_lens), max_query_len,
+            d ** -0.5 if scale is None else float(scale), lse.data_ptr(), lse.stride(0),
+            None if row_factors is None else row_factors.data_ptr(),
+            0 if row_factors is None else row_factors.stride(0),
+            weights.data_ptr(), weights.stride(0), weights.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1), weights.shape[2],
+            _lib.stream_ptr(dev)), what)
+    return out
 
 
 def cache_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -154,4 +214,4 @@ def cache_evict(weights: torch.Tensor, seq_lens: torch.Tensor, block_table: torc
     return kept, lengths
 
 
-__all__ = ["cache_compact", "cache_evict", "cache_evict_workspace_bytes"]
+__all__ = ["accumulate_attention_weights", "cache_compact", "cache_evict", "cache_evict_workspace_bytes"]
