@@ -370,6 +370,12 @@ __device__ __forceinline__ bool tree_sees(const TreeParams& p, const TreeRequest
 cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t stream);
 size_t tree_attention_workspace(int rows, int requests, int q_heads, int kv_heads, int dim,
                                 int max_query_len);
+// tcgen05 + TMA form (tree_attention_tc.cu): launch_tree_attention takes it
+// where tree_attention_tc_eligible() holds and the strides can be described to
+// the TMA unit (else cudaErrorNotSupported, nothing launched).
+bool tree_attention_tc_eligible(const TreeParams& p);
+cudaError_t launch_tree_attention_tc(const TreeParams& p, cudaStream_t stream);
+size_t tree_attention_tc_workspace(int group, int dim, int max_query_len);
 cudaError_t launch_attention_weights(const TreeParams& p, cudaStream_t stream);
 
 int num_sms();

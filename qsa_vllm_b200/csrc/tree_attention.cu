@@ -240,10 +240,14 @@ __global__ void __launch_bounds__(kGenThreads) attention_weights_general(TreePar
 
 size_t tree_attention_workspace(int rows, int requests, int q_heads, int kv_heads, int dim,
                                 int max_query_len) {
-  return 0;
+  return tree_attention_tc_workspace(q_heads / kv_heads, dim, max_query_len);
 }
 
 cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t stream) {
+  if (tree_attention_tc_eligible(p)) {
+    const cudaError_t e = launch_tree_attention_tc(p, stream);
+    if (e != cudaErrorNotSupported) return e;
+  }
   return count_launches(launch_kernel(tree_attention_general, dim3(p.rows, p.kv_heads),
                                       dim3(kGenThreads), 0, stream, 1, p));
 }
