@@ -14,7 +14,7 @@
 // have the same rows and take alternate token tiles, joined at the end.
 //
 // Roles: warp 0 loads query, key and value tiles page by page with TMA into a
-// ring; one thread of warp 1 issues all tensor-core work; warps 4-7 and 8-11
+// ring; one thread of warp 1 issues all tensor-core work; warps 2-5 and 6-9
 // are the softmax warpgroups, one thread per row of S (a TMEM lane).
 //  * The maximum that p is taken against moves only when it would let p pass
 //    2^8 (rescaling O costs a round trip through TMEM); sums stay below 2^24
@@ -50,7 +50,9 @@
 namespace qsa {
 namespace {
 
-constexpr int kTreeThreads = 384;
+// 10 warps: 200 registers a thread, what the softmax warps need without spills
+// (which would go to L2: shared memory leaves hardly any L1)
+constexpr int kTreeThreads = 320;
 constexpr int kTile = 128;          // tokens per tile, and rows per row tile
 constexpr int kMetaRing = 8;
 constexpr int kTmemCols = 512;      // S0 S1 O0 O1
@@ -261,6 +263,101 @@ __device__ __forceinline__ float unpack(uint16_t x) {
   else return __uint_as_float(static_cast<uint32_t>(x) << 16);
 }
 
+// ------------------------------------------------------------------ softmax
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+      "%13,%14,%15};" ::QSA_I8(r, 0),
+      QSA_I8(r, 8), "r"(taddr)
+      : "memory");
+}
+
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+
+__device__ __forceinline__ void hide32(uint32_t* s, uint32_t seen) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k)
+    if (!((seen >> k) & 1)) s[k] = 0xff800000u;  // -inf
+}
+
+__device__ __forceinline__ float max64(const uint32_t* s) {
+  float h[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) h[q] = __uint_as_float(s[q]);
+#pragma unroll
+  for (int k = 4; k + 8 <= 64; k += 8)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      h[q] = fmaxf(fmaxf(h[q], __uint_as_float(s[k + q])), __uint_as_float(s[k + 4 + q]));
+#pragma unroll
+  for (int q = 0; q < 4; ++q) h[q] = fmaxf(h[q], __uint_as_float(s[60 + q]));
+  return fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3]));
+}
+
+// s[0..15] <- the 32 exponentials as 16-bit pairs; their 32-bit values are
+// added to `sum`.
+template <bool F16>
+__device__ __forceinline__ void exp_pairs(uint32_t* s, float c, float shift, float2& sum) {
+  const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
+#pragma unroll
+  for (int k = 0; k < 32; k += 2) {
+    float2 x = fma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, shift2);
+    x.x = fast_exp2(x.x);
+    x.y = fast_exp2(x.y);
+    sum = add2(sum, x);
+    s[k / 2] = pack2<F16>(x.x, x.y);
+  }
+}
+
+// Clears the bits of tile t's columns that row i of the request does not see.
+// Collective over the warp, whose lanes hold the rows i0 + local.
+__device__ __forceinline__ void row_mask(uint32_t (&w)[4], const TreeParams& p,
+                                         const TreeRequest& r, int t, int i, int i0, int local,
+                                         int R, int lane) {
+  const int node0 = t * kTile - r.prefix;  // drafted token of column 0
+  if (p.mask == nullptr) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int see = i - node0 - k * 32 + 1;  // columns of this word that are seen
+      w[k] &= see >= 32 ? 0xffffffffu : see <= 0 ? 0u : (1u << see) - 1;
+    }
+    return;
+  }
+  // the distinct rows of this warp, one after another: 128 mask bytes read
+  // side by side, turned into bits by ballots
+  const int lo = __shfl_sync(0xffffffffu, local, 0);
+  const int hi = min(__shfl_sync(0xffffffffu, local, 31), R - 1);
+  uint32_t sees[4] = {0u, 0u, 0u, 0u};
+  for (int k = lo; k <= hi; ++k) {
+    if (i0 + k >= r.count) break;
+    const uint8_t* bytes = p.mask + (r.row0 + i0 + k) * p.mask_stride;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int node = node0 + q * 32 + lane;
+      const bool see = node < 0 || (node < p.mask_width && bytes[node] != 0);
+      const uint32_t bits = __ballot_sync(0xffffffffu, see);
+      if (k == local) sees[q] = bits;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] &= sees[k];
+}
+
 // --------------------------------------------------------------- the kernel
 template <int D, bool DUAL, bool F16>
 __global__ void __launch_bounds__(kTreeThreads, 1)
@@ -379,11 +476,6 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     if (*reinterpret_cast<volatile int*>(&sm.abort_flag)) return false;
     return mbar_wait(bar, parity);
   };
-
-  // 384 threads are launched with 168 registers each; 128 x 88 + 256 x 208 is
-  // as many
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -556,9 +648,9 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
       }
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------------------- softmax
-    const int st = warp >= 8 ? 1 : 0;
+    const int st = warp >= 6 ? 1 : 0;
     const int quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t ts = tmem_s[st] + lane_off, to = tmem_o[st] + lane_off;
@@ -586,84 +678,11 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         if (!ok) break;
         ++tiles_done;
         tc_fence_after();
-        uint32_t sr[kTile];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tmem_ld32(ts + k * 32, sr + k * 32);
         const uint4 words = *reinterpret_cast<const uint4*>(sm.meta[seq % kMetaRing]);
-        const bool masked = (t + 1) * kTile > region ||
-                            (words.x & words.y & words.z & words.w) != 0xffffffffu;
-        tmem_wait_ld();
+        uint32_t w[4] = {words.x, words.y, words.z, words.w};
+        const bool masked = (t + 1) * kTile > region || (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu;
         if (masked) {
-          uint32_t w[4] = {words.x, words.y, words.z, words.w};
-          const int node0 = t * kTile - r.prefix;  // drafted token of column 0
-          if (p.mask == nullptr) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int see = i - node0 - k * 32 + 1;  // columns of this word that are seen
-              w[k] &= see >= 32 ? 0xffffffffu : see <= 0 ? 0u : (1u << see) - 1;
-            }
-          } else {
-            // the distinct rows of this warp, one after another: 128 mask bytes
-            // read side by side, turned into bits by ballots
-            const int lo = __shfl_sync(0xffffffffu, local, 0);
-            const int hi = min(__shfl_sync(0xffffffffu, local, 31), R - 1);
-            uint32_t sees[4] = {0u, 0u, 0u, 0u};
-            for (int k = lo; k <= hi; ++k) {
-              if (i0 + k >= r.count) break;
-              const uint8_t* bytes = p.mask + (r.row0 + i0 + k) * p.mask_stride;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const int node = node0 + q * 32 + lane;
-                const bool see = node < 0 || (node < p.mask_width && bytes[node] != 0);
-                const uint32_t bits = __ballot_sync(0xffffffffu, see);
-                if (k == local) sees[q] = bits;
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] &= sees[k];
-          }
-#pragma unroll
-          for (int k = 0; k < kTile; ++k)
-            if (!((w[k / 32] >> (k % 32)) & 1)) sr[k] = 0xff800000u;  // -inf
-        }
-        float high = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < kTile; k += 2)
-          high = fmaxf(high, fmaxf(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])));
-        if (fresh) {
-          m = high;
-        } else {
-          const bool move = high > m && (m == -INFINITY || (high - m) * c > kSlack);
-          if (__any_sync(0xffffffffu, move)) {
-            // the products so far are done: this S was issued behind them
-            const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : fast_exp2((m - high) * c);
-            if (move) m = high;
-            l *= f;
-#pragma unroll
-            for (int k = 0; k < D; k += 32) {
-              uint32_t o[32];
-              tmem_ld32(to + k, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(to + k, o);
-            }
-          }
-        }
-        fresh = false;
-        const float shift = m == -INFINITY ? 0.0f : -m * c;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < kTile; k += 2) {
-          const float a = fast_exp2(fmaf(__uint_as_float(sr[k]), c, shift));
-          const float b = fast_exp2(fmaf(__uint_as_float(sr[k + 1]), c, shift));
-          sum[k / 2 % 4] += a + b;
-          sr[k / 2] = pack2<F16>(a, b);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st32(ts, sr);
-        tmem_st32(ts + 32, sr + 32);
-        if (masked) {
+          row_mask(w, p, r, t, i, i0, local, R, lane);
           // Values of tokens that may not be read become 0; infinite or NaN
           // elements of drafted tokens too, and the piece remembers them.
           const int vseq = 2 * seq + 1;
@@ -672,12 +691,12 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
           constexpr int kParts = DUAL ? 2 : 1;   // threads of one token
           const int token = DUAL ? st * 64 + row / 2 : row;
           const int part = DUAL ? row & 1 : 0;
-          const uint32_t word = reinterpret_cast<const uint32_t*>(&words)[token / 32];
+          const uint32_t word = sm.meta[seq % kMetaRing][token / 32];
           const bool exists = (word >> (token % 32)) & 1;
           uint4* v = reinterpret_cast<uint4*>(sm.ring[vseq % C::S]);
           constexpr int kChunks = C::kSub * 8 / kParts;  // 16-byte chunks of this thread
           if (!exists || t * kTile + token >= region) {
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < kChunks; ++k) {
               const int at = part * kChunks + k;
               uint4* x = v + (at / 8) * (C::kSubBytes / 16) + token * 8 + at % 8;
@@ -706,6 +725,55 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             ++vsyncs;
           }
         }
+        // The scores are read twice, the maximum first: all 128 beside the rest
+        // would not fit the registers.
+        float high = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t sr[64];
+          tmem_ld32(ts + k * 64, sr);
+          tmem_ld32(ts + k * 64 + 32, sr + 32);
+          tmem_wait_ld();
+          if (masked) {
+            hide32(sr, w[2 * k]);
+            hide32(sr + 32, w[2 * k + 1]);
+          }
+          high = fmaxf(high, max64(sr));
+        }
+        if (fresh) {
+          m = high;
+        } else {
+          const bool move = high > m && (m == -INFINITY || (high - m) * c > kSlack);
+          if (__any_sync(0xffffffffu, move)) {
+            // the products so far are done: this S was issued behind them
+            const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : fast_exp2((m - high) * c);
+            if (move) m = high;
+            l *= f;
+#pragma unroll
+            for (int k = 0; k < D; k += 16) {
+              uint32_t o[16];
+              tmem_ld16(to + k, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(to + k, o);
+            }
+          }
+        }
+        fresh = false;
+        const float shift = m == -INFINITY ? 0.0f : -m * c;
+        float2 sum = make_float2(0.0f, 0.0f);
+        uint32_t sr[2][32];
+        tmem_ld32(ts, sr[0]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          tmem_wait_ld();
+          if (k < 3) tmem_ld32(ts + (k + 1) * 32, sr[(k + 1) & 1]);
+          if (masked) hide32(sr[k & 1], w[k]);
+          exp_pairs<F16>(sr[k & 1], c, shift, sum);
+          tmem_st16(ts + k * 16, sr[k & 1]);  // over scores that have been read
+        }
+        l += sum.x + sum.y;
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sm.p_ready[st]);
