@@ -14,7 +14,7 @@
 // have the same rows and take alternate token tiles, joined at the end.
 //
 // Roles: warp 0 loads query, key and value tiles page by page with TMA into a
-// ring; one thread of warp 1 issues all tensor-core work; warps 2-5 and 6-9
+// ring; one lane of warp 1 issues all tensor-core work; warps 2-5 and 6-9
 // are the softmax warpgroups, one thread per row of S (a TMEM lane).
 //  * The maximum that p is taken against moves only when it would let p pass
 //    2^8 (rescaling O costs a round trip through TMEM); sums stay below 2^24
@@ -192,6 +192,29 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t saddr) {
   return d;
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
+// A place in the ring of key and value tiles, which alternate.
+struct RingPos {
+  int slot;
+  uint32_t phase;
+  template <int S>
+  __device__ __forceinline__ void step() {
+    slot += 2;
+    if (slot >= S) {
+      slot -= S;
+      phase ^= 1;
+    }
+  }
+};
+
 // D += A(TMEM) * B(shared memory).
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
                                         uint32_t idesc, bool accumulate) {
@@ -295,24 +318,24 @@ __device__ __forceinline__ void hide32(uint32_t* s, uint32_t seen) {
     if (!((seen >> k) & 1)) s[k] = 0xff800000u;  // -inf
 }
 
-__device__ __forceinline__ float max64(const uint32_t* s) {
+__device__ __forceinline__ float max32(const uint32_t* s) {
   float h[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) h[q] = __uint_as_float(s[q]);
 #pragma unroll
-  for (int k = 4; k + 8 <= 64; k += 8)
+  for (int k = 4; k + 8 <= 32; k += 8)
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       h[q] = fmaxf(fmaxf(h[q], __uint_as_float(s[k + q])), __uint_as_float(s[k + 4 + q]));
 #pragma unroll
-  for (int q = 0; q < 4; ++q) h[q] = fmaxf(h[q], __uint_as_float(s[60 + q]));
+  for (int q = 0; q < 4; ++q) h[q] = fmaxf(h[q], __uint_as_float(s[28 + q]));
   return fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3]));
 }
 
-// s[0..15] <- the 32 exponentials as 16-bit pairs; their 32-bit values are
-// added to `sum`.
+// pk <- 32 exponentials as 16-bit pairs; their 32-bit values are added to `sum`.
 template <bool F16>
-__device__ __forceinline__ void exp_pairs(uint32_t* s, float c, float shift, float2& sum) {
+__device__ __forceinline__ void exp_pairs(const uint32_t* s, uint32_t* pk, float c, float shift,
+                                          float2& sum) {
   const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
 #pragma unroll
   for (int k = 0; k < 32; k += 2) {
@@ -320,7 +343,7 @@ __device__ __forceinline__ void exp_pairs(uint32_t* s, float c, float shift, flo
     x.x = fast_exp2(x.x);
     x.y = fast_exp2(x.y);
     sum = add2(sum, x);
-    s[k / 2] = pack2<F16>(x.x, x.y);
+    pk[k / 2] = pack2<F16>(x.x, x.y);
   }
 }
 
@@ -554,98 +577,114 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     __syncwarp();
   } else if (warp == 1) {
     // -------------------------------------------------------- tensor cores
-    if (lane == 0) {
-      constexpr uint32_t kQk = tree_idesc<F16, kTile, false>();
-      constexpr uint32_t kPv = tree_idesc<F16, D, true>();
-      int n = 0, piece = 0;
-      uint32_t given[2] = {0, 0};  // P tiles taken of each softmax warpgroup
-      auto qk = [&](int s, int seq_n) {
-        const uint32_t a = smem_u32(sm.q[DUAL ? s : 0]);
-        const uint32_t b = smem_u32(sm.ring[(2 * seq_n) % C::S]);
+    // The whole warp keeps the loop (descriptors then stay in uniform
+    // registers); one elected lane issues.
+    constexpr uint32_t kQk = tree_idesc<F16, kTile, false>();
+    constexpr uint32_t kPv = tree_idesc<F16, D, true>();
+    const bool leader = elect_lane();
+    const uint64_t q_desc = sw128_desc(smem_u32(sm.q[0]));
+    const uint64_t k_desc = sw128_desc(smem_u32(sm.ring[0]));
+    const uint64_t v_desc = value_desc(smem_u32(sm.ring[0]));
+    int piece = 0;
+    uint32_t given[2] = {0, 0};  // P tiles taken of each softmax warpgroup
+    RingPos kp{0, 0}, vp{1, 0};
+    auto qk = [&](int s) {
+      if (leader) {
+        const uint64_t a = q_desc + (DUAL ? s : 0) * (C::kTileBytes >> 4);
+        const uint64_t b = k_desc + static_cast<uint32_t>(kp.slot) * (C::kTileBytes >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * C::kSubBytes + (k % 4) * 32;
-          umma_bf16(tmem_s[s], sw128_desc(a + off), sw128_desc(b + off), kQk, k > 0);
+          const uint32_t off = ((k / 4) * C::kSubBytes + (k % 4) * 32) >> 4;
+          umma_bf16(tmem_s[s], a + off, b + off, kQk, k > 0);
         }
         umma_commit(&sm.s_full[s]);
-      };
-      auto pv = [&](int s, int seq_n, bool accumulate) {
-        const uint32_t b = smem_u32(sm.ring[(2 * seq_n + 1) % C::S]);
+      }
+    };
+    auto pv = [&](int s, bool accumulate) {
+      if (leader) {
+        const uint64_t b = v_desc + static_cast<uint32_t>(vp.slot) * (C::kTileBytes >> 4);
 #pragma unroll
         for (int k = 0; k < kTile / 16; ++k)
-          umma_ts(tmem_o[s], tmem_s[s] + k * 8, value_desc(b + k * 2048), kPv,
-                  accumulate || k > 0);
-      };
-      auto k_in = [&](int seq_n) {
-        const int seq = 2 * seq_n;
-        return wait(&sm.full[seq % C::S], (seq / C::S) & 1);
-      };
-      auto v_in = [&](int seq_n) {
-        const int seq = 2 * seq_n + 1;
-        return wait(&sm.full[seq % C::S], (seq / C::S) & 1);
-      };
-      auto p_in = [&](int s) { return wait(&sm.p_ready[s], given[s]++ & 1); };
-      for (; ok && u.base < end; ++piece) {
-        const int t0 = static_cast<int>(max(begin - u.base, static_cast<int64_t>(0)));
-        const int t1 = static_cast<int>(min(end - u.base, static_cast<int64_t>(u.tiles)));
-        const int m = t1 - t0;
-        ok = wait(&sm.q_full, piece & 1);
-        if (!ok) break;
-        if constexpr (DUAL) {
-          for (int j = 0; j <= m && ok; ++j) {
+          umma_ts(tmem_o[s], tmem_s[s] + k * 8, b + ((k * 2048) >> 4), kPv, accumulate || k > 0);
+      }
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+    };
+    auto arrived = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, wait(bar, parity));
+    };
+    auto k_in = [&]() { return arrived(&sm.full[kp.slot], kp.phase); };
+    auto v_in = [&]() { return arrived(&sm.full[vp.slot], vp.phase); };
+    auto p_in = [&](int s) { return arrived(&sm.p_ready[s], given[s]++ & 1); };
+    for (; ok && u.base < end; ++piece) {
+      const int t0 = static_cast<int>(max(begin - u.base, static_cast<int64_t>(0)));
+      const int t1 = static_cast<int>(min(end - u.base, static_cast<int64_t>(u.tiles)));
+      const int m = t1 - t0;
+      ok = arrived(&sm.q_full, piece & 1);
+      if (!ok) break;
+      if constexpr (DUAL) {
+        for (int j = 0; j <= m && ok; ++j) {  // product j - 1, then scores j
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              if (j > 0) {
-                ok = ok && (s || v_in(n + j - 1)) && p_in(s);
-                if (!ok) break;
-                tc_fence_after();
-                pv(s, n + j - 1, j > 1);
-              }
-              if (j < m) {
-                ok = ok && (s || k_in(n + j));
-                if (!ok) break;
-                tc_fence_after();
-                qk(s, n + j);
-              } else {
-                umma_commit(&sm.o_full[s]);
-              }
-            }
-            if (!ok) break;
-            if (j > 0) umma_commit(&sm.empty[(2 * (n + j - 1) + 1) % C::S]);
-            if (j < m) umma_commit(&sm.empty[(2 * (n + j)) % C::S]);
-            if (j == m - 1) umma_commit(&sm.q_empty);
-          }
-        } else {
-          for (int j = 0; j < m + 2 && ok; ++j) {  // product j - 2, then scores j
-            if (j >= 2) {
-              ok = v_in(n + j - 2) && p_in(j & 1);
+          for (int s = 0; s < 2; ++s) {
+            if (j > 0) {
+              ok = ok && (s || v_in()) && p_in(s);
               if (!ok) break;
               tc_fence_after();
-              pv(j & 1, n + j - 2, j >= 4);
-              umma_commit(&sm.empty[(2 * (n + j - 2) + 1) % C::S]);
+              pv(s, j > 1);
             }
             if (j < m) {
-              ok = k_in(n + j);
+              ok = ok && (s || k_in());
               if (!ok) break;
               tc_fence_after();
-              qk(j & 1, n + j);
-              umma_commit(&sm.empty[(2 * (n + j)) % C::S]);
-              if (j == m - 1) umma_commit(&sm.q_empty);
+              qk(s);
+            } else {
+              commit(&sm.o_full[s]);
             }
           }
           if (!ok) break;
-          umma_commit(&sm.o_full[0]);
-          umma_commit(&sm.o_full[1]);
+          if (j > 0) {
+            commit(&sm.empty[vp.slot]);
+            vp.template step<C::S>();
+          }
+          if (j < m) {
+            commit(&sm.empty[kp.slot]);
+            kp.template step<C::S>();
+          }
+          if (j == m - 1) commit(&sm.q_empty);
+        }
+      } else {
+        for (int j = 0; j < m + 2 && ok; ++j) {  // product j - 2, then scores j
+          const int s = j & 1;
+          if (j >= 2) {
+            ok = v_in() && p_in(s);
+            if (!ok) break;
+            tc_fence_after();
+            pv(s, j >= 4);
+            commit(&sm.empty[vp.slot]);
+            vp.template step<C::S>();
+          }
+          if (j < m) {
+            ok = k_in();
+            if (!ok) break;
+            tc_fence_after();
+            qk(s);
+            commit(&sm.empty[kp.slot]);
+            kp.template step<C::S>();
+            if (j == m - 1) commit(&sm.q_empty);
+          }
         }
         if (!ok) break;
-        n += m;
-        if (!unit_next(p, u, span)) break;
+        commit(&sm.o_full[0]);
+        commit(&sm.o_full[1]);
       }
-      if (!ok) {
-        give_up();
-        umma_commit(&sm.drain);  // products in flight end before the block may
-        mbar_wait(&sm.drain, 0);
-      }
+      if (!ok) break;
+      if (!unit_next(p, u, span)) break;
+    }
+    if (!ok) {
+      if (lane == 0) give_up();
+      commit(&sm.drain);  // products in flight end before the block may
+      mbar_wait(&sm.drain, 0);
     }
     __syncwarp();
   } else {
@@ -725,29 +764,35 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             ++vsyncs;
           }
         }
-        // The scores are read twice, the maximum first: all 128 beside the rest
-        // would not fit the registers.
-        float high = -INFINITY;
+        // One pass over the scores takes their maximum and, against the
+        // maximum so far, their exponentials.  Where the new maximum lies too
+        // far above (always in a piece's first tile, rarely later) it becomes
+        // the one to take them against, and the pass is made again: S is
+        // still whole, as P is only written behind this loop.
+        uint32_t pk[kTile / 2];
+        float2 sum;
+        for (bool settled = false;;) {
+          const float shift = m == -INFINITY ? 0.0f : -m * c;
+          float high = -INFINITY;
+          sum = make_float2(0.0f, 0.0f);
+          uint32_t sr[2][32];
+          tmem_ld32(ts, sr[0]);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t sr[64];
-          tmem_ld32(ts + k * 64, sr);
-          tmem_ld32(ts + k * 64 + 32, sr + 32);
-          tmem_wait_ld();
-          if (masked) {
-            hide32(sr, w[2 * k]);
-            hide32(sr + 32, w[2 * k + 1]);
+          for (int k = 0; k < 4; ++k) {
+            tmem_wait_ld();
+            if (k < 3) tmem_ld32(ts + (k + 1) * 32, sr[(k + 1) & 1]);
+            if (masked) hide32(sr[k & 1], w[k]);
+            high = fmaxf(high, max32(sr[k & 1]));
+            exp_pairs<F16>(sr[k & 1], pk + k * 16, c, shift, sum);
           }
-          high = fmaxf(high, max64(sr));
-        }
-        if (fresh) {
-          m = high;
-        } else {
-          const bool move = high > m && (m == -INFINITY || (high - m) * c > kSlack);
-          if (__any_sync(0xffffffffu, move)) {
+          if (settled) break;
+          const bool move =
+              fresh || (high > m && (m == -INFINITY || (high - m) * c > kSlack));
+          if (!__any_sync(0xffffffffu, move)) break;
+          settled = true;
+          if (!fresh) {
             // the products so far are done: this S was issued behind them
             const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : fast_exp2((m - high) * c);
-            if (move) m = high;
             l *= f;
 #pragma unroll
             for (int k = 0; k < D; k += 16) {
@@ -759,20 +804,11 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
               tmem_st16(to + k, o);
             }
           }
+          if (move) m = high;
+          fresh = false;
         }
-        fresh = false;
-        const float shift = m == -INFINITY ? 0.0f : -m * c;
-        float2 sum = make_float2(0.0f, 0.0f);
-        uint32_t sr[2][32];
-        tmem_ld32(ts, sr[0]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          tmem_wait_ld();
-          if (k < 3) tmem_ld32(ts + (k + 1) * 32, sr[(k + 1) & 1]);
-          if (masked) hide32(sr[k & 1], w[k]);
-          exp_pairs<F16>(sr[k & 1], c, shift, sum);
-          tmem_st16(ts + k * 16, sr[k & 1]);  // over scores that have been read
-        }
+        tmem_st32(ts, pk);
+        tmem_st32(ts + 32, pk + 32);
         l += sum.x + sum.y;
         tmem_wait_st();
         tc_fence_before();
