@@ -90,13 +90,28 @@ struct TreeCfg {
   static constexpr int kRows = kStreams * kTile;
 };
 
+// A unit's part inside a CTA's range, handed by the producer to the others.
+struct TreePiece {
+  TreeRequest r;
+  int b, h;
+  int first;   // the CTA's first row of the request
+  int region;  // tokens from here on are not seen by all of its rows
+  int t0, t1;  // token tiles
+  int tiles;   // of the whole unit
+  int end;     // no more pieces
+};
+// A piece's slot is written again four pieces later, when the products of the
+// piece three later have been issued and its softmax is two pieces past it.
+constexpr int kPieceRing = 4;
+
 template <int D, bool DUAL>
 struct TreeSmem {
   using C = TreeCfg<D, DUAL>;
   alignas(1024) uint8_t ring[C::S][C::kTileBytes];    // key and value tiles, 128B-swizzled
   alignas(1024) uint8_t q[C::kStreams][C::kTileBytes];
   uint64_t full[C::S], empty[C::S], q_full, q_empty, s_full[2], p_ready[2], o_full[2];
-  uint64_t vsync, xchg[2], drain;
+  uint64_t vsync, xchg[2], drain, piece_full[kPieceRing];
+  TreePiece piece[kPieceRing];
   alignas(16) uint32_t meta[kMetaRing][4];  // tokens of the tile that exist on mapped pages
   float2 ml[kTile];              // (m, l) of the second softmax warpgroup
   int64_t scan[kTreeThreads / 32];
@@ -312,51 +327,54 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&d);
 }
 
-__device__ __forceinline__ void hide32(uint32_t* s, uint32_t seen) {
-#pragma unroll
-  for (int k = 0; k < 32; ++k)
-    if (!((seen >> k) & 1)) s[k] = 0xff800000u;  // -inf
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
-
-__device__ __forceinline__ float max32(const uint32_t* s) {
-  float h[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) h[q] = __uint_as_float(s[q]);
-#pragma unroll
-  for (int k = 4; k + 8 <= 32; k += 8)
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      h[q] = fmaxf(fmaxf(h[q], __uint_as_float(s[k + q])), __uint_as_float(s[k + 4 + q]));
-#pragma unroll
-  for (int q = 0; q < 4; ++q) h[q] = fmaxf(h[q], __uint_as_float(s[28 + q]));
-  return fmaxf(fmaxf(h[0], h[1]), fmaxf(h[2], h[3]));
-}
-
-// pk <- 32 exponentials as 16-bit pairs; their 32-bit values are added to `sum`.
+// One pass over a row's 128 scores: their maximum (returned), and against m
+// their exponentials, as 16-bit pairs in pk, and the sum of those in 32 bits.
+// The special-function unit takes 8 cycles for a warp's exponential, 1024 for
+// the row, the rest about half of that: a pass alone on its scheduler takes
+// 1550 cycles, two at once 2400.
 template <bool F16>
-__device__ __forceinline__ void exp_pairs(const uint32_t* s, uint32_t* pk, float c, float shift,
-                                          float2& sum) {
+__device__ __forceinline__ float score_pass(uint32_t ts, float c, float m, uint32_t* pk,
+                                            float2& sum) {
+  const float shift = m == -INFINITY ? 0.0f : -m * c;
   const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
+  float high = -INFINITY;
+  sum = make_float2(0.0f, 0.0f);
+  uint32_t s[2][32];
+  tmem_ld32(ts, s[0]);
 #pragma unroll
-  for (int k = 0; k < 32; k += 2) {
-    float2 x = fma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, shift2);
-    x.x = fast_exp2(x.x);
-    x.y = fast_exp2(x.y);
-    sum = add2(sum, x);
-    pk[k / 2] = pack2<F16>(x.x, x.y);
+  for (int k = 0; k < 4; ++k) {
+    tmem_wait_ld();
+    if (k < 3) tmem_ld32(ts + (k + 1) * 32, s[(k + 1) & 1]);
+    uint32_t* v = s[k & 1];
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float a = __uint_as_float(v[e]), b = __uint_as_float(v[e + 1]);
+      float2 x = fma2(make_float2(a, b), c2, shift2);
+      x.x = fast_exp2(x.x);
+      x.y = fast_exp2(x.y);
+      high = max3(high, a, b);
+      sum = add2(sum, x);
+      pk[k * 16 + e / 2] = pack2<F16>(x.x, x.y);
+    }
   }
+  return high;
 }
 
-// Clears the bits of tile t's columns that row i of the request does not see.
-// Collective over the warp, whose lanes hold the rows i0 + local.
+// Clears the bits of tile t's columns that row i0 + local of the request does
+// not see.  Collective over the warp.
 __device__ __forceinline__ void row_mask(uint32_t (&w)[4], const TreeParams& p,
-                                         const TreeRequest& r, int t, int i, int i0, int local,
-                                         int R, int lane) {
+                                         const TreeRequest& r, int t, int i0, int local, int R,
+                                         int lane) {
   const int node0 = t * kTile - r.prefix;  // drafted token of column 0
   if (p.mask == nullptr) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int see = i - node0 - k * 32 + 1;  // columns of this word that are seen
+      const int see = i0 + local - node0 - k * 32 + 1;  // columns of this word that are seen
       w[k] &= see >= 32 ? 0xffffffffu : see <= 0 ? 0u : (1u << see) - 1;
     }
     return;
@@ -406,11 +424,12 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     mbar_init(&sm.q_empty, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sm.s_full[s], 1);
-      mbar_init(&sm.p_ready[s], kTile);
+      mbar_init(&sm.p_ready[s], 4);
       mbar_init(&sm.o_full[s], 1);
       mbar_init(&sm.xchg[s], kTile);
       sm.bad[s] = -1;
     }
+    for (int s = 0; s < kPieceRing; ++s) mbar_init(&sm.piece_full[s], 1);
     mbar_init(&sm.vsync, 2 * kTile);
     mbar_init(&sm.drain, 1);
     sm.abort_flag = 0;
@@ -485,17 +504,13 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
   const uint32_t tmem = sm.tmem_base;
   const uint32_t tmem_s[2] = {tmem, tmem + 128}, tmem_o[2] = {tmem + 256, tmem + 384};
 
-  TreeUnit u;
-  bool ok = unit_seek(p, u, sm.first_b, sm.first_base, begin, span);
-  if (tid == 0) {
-    PieceInfo info = {total, u.base, u.tiles, u.b, u.h, u.grp, ranges, begin > u.base};
-    g.info[blockIdx.x] = info;
-  }
+  bool ok = true;
   auto give_up = [&]() {
     record_error(p.err, kDeviceErrWaitTimeout);
     *reinterpret_cast<volatile int*>(&sm.abort_flag) = 1;
   };
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(&sm.abort_flag)) return false;
     return mbar_wait(bar, parity);
   };
@@ -505,19 +520,34 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     int n = 0, piece = 0;  // tiles and pieces so far
     const int boxes = kTile / g.box_rows;
     const uint32_t box_bytes = g.box_rows * 128;
-    for (; ok && u.base < end; ++piece) {
+    TreeUnit u;
+    bool more = unit_seek(p, u, sm.first_b, sm.first_base, begin, span);
+    if (lane == 0) {
+      PieceInfo info = {total, u.base, u.tiles, u.b, u.h, u.grp, ranges, begin > u.base};
+      g.info[blockIdx.x] = info;
+    }
+    for (;; ++piece) {
+      more = more && u.base < end;
       const int t0 = static_cast<int>(max(begin - u.base, static_cast<int64_t>(0)));
       const int t1 = static_cast<int>(min(end - u.base, static_cast<int64_t>(u.tiles)));
+      const int first = (u.grp * g.cohort + member) * C::kStreams * R;
       ok = __all_sync(0xffffffffu, wait(&sm.q_empty, (piece & 1) ^ 1));
       if (!ok) break;
+      if (lane == 0) {
+        const int region =
+            max(p.mask != nullptr ? u.r.prefix : u.r.prefix + first + 1, 0);
+        sm.piece[piece % kPieceRing] =
+            TreePiece{u.r, u.b, u.h, first, region, t0, t1, u.tiles, !more};
+        mbar_arrive(&sm.piece_full[piece % kPieceRing]);
+      }
+      if (!more) break;
       if (lane == 0) {
         const int rows = R * p.group;
         mbar_arrive_expect(&sm.q_full, C::kStreams * C::kSub * rows * 128);
         for (int s = 0; s < C::kStreams; ++s)
           for (int c = 0; c < C::kSub; ++c)
             tma_load_4d(sm.q[s] + c * C::kSubBytes, &qmap, c * 64, 0, u.h,
-                        u.r.row0 + (u.grp * g.cohort + member) * C::kStreams * R + s * R,
-                        &sm.q_full);
+                        u.r.row0 + first + s * R, &sm.q_full);
       }
       const int32_t* table = p.table + u.b * p.table_stride;
       auto page_of = [&](int tile, int& at) {
@@ -565,7 +595,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         }
         if (!ok) break;
       }
-      if (!ok || !unit_next(p, u, span)) break;
+      if (!ok) break;
+      more = unit_next(p, u, span);
     }
     if (!ok && lane == 0) give_up();
     // copies in flight end before the block may
@@ -612,15 +643,16 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
       if (leader) umma_commit(bar);
     };
     auto arrived = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, wait(bar, parity));
+      return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
     };
     auto k_in = [&]() { return arrived(&sm.full[kp.slot], kp.phase); };
     auto v_in = [&]() { return arrived(&sm.full[vp.slot], vp.phase); };
     auto p_in = [&](int s) { return arrived(&sm.p_ready[s], given[s]++ & 1); };
-    for (; ok && u.base < end; ++piece) {
-      const int t0 = static_cast<int>(max(begin - u.base, static_cast<int64_t>(0)));
-      const int t1 = static_cast<int>(min(end - u.base, static_cast<int64_t>(u.tiles)));
-      const int m = t1 - t0;
+    for (;; ++piece) {
+      const TreePiece& pc = sm.piece[piece % kPieceRing];
+      ok = arrived(&sm.piece_full[piece % kPieceRing], piece / kPieceRing & 1);
+      if (!ok || pc.end) break;
+      const int m = pc.t1 - pc.t0;
       ok = arrived(&sm.q_full, piece & 1);
       if (!ok) break;
       if constexpr (DUAL) {
@@ -628,13 +660,13 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             if (j > 0) {
-              ok = ok && (s || v_in()) && p_in(s);
+              ok = ok && (s || (v_in() && (j == m || k_in()))) && p_in(s);
               if (!ok) break;
               tc_fence_after();
               pv(s, j > 1);
             }
             if (j < m) {
-              ok = ok && (s || k_in());
+              if (j == 0) ok = ok && (s || k_in());
               if (!ok) break;
               tc_fence_after();
               qk(s);
@@ -657,7 +689,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         for (int j = 0; j < m + 2 && ok; ++j) {  // product j - 2, then scores j
           const int s = j & 1;
           if (j >= 2) {
-            ok = v_in() && p_in(s);
+            ok = v_in() && (j >= m || k_in()) && p_in(s);
             if (!ok) break;
             tc_fence_after();
             pv(s, j >= 4);
@@ -665,7 +697,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             vp.template step<C::S>();
           }
           if (j < m) {
-            ok = k_in();
+            if (j < 2) ok = k_in();
             if (!ok) break;
             tc_fence_after();
             qk(s);
@@ -679,7 +711,6 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         commit(&sm.o_full[1]);
       }
       if (!ok) break;
-      if (!unit_next(p, u, span)) break;
     }
     if (!ok) {
       if (lane == 0) give_up();
@@ -696,18 +727,15 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     const float c = p.scale_log2;
     int n = 0, piece = 0;
     uint32_t tiles_done = 0, vsyncs = 0;
-    int local, head;
-    g.group_div.divmod(row, local, head);
-    for (; ok && u.base < end; ++piece) {
-      const int t0 = static_cast<int>(max(begin - u.base, static_cast<int64_t>(0)));
-      const int t1 = static_cast<int>(min(end - u.base, static_cast<int64_t>(u.tiles)));
-      const TreeRequest r = u.r;
-      const int first = (u.grp * g.cohort + member) * C::kStreams * R;  // the CTA's first row
-      const int i0 = first + (DUAL ? st * R : 0);
-      const int i = i0 + local;                       // this thread's row of the request
-      const bool live = local < R && i < r.count;
-      // tokens from here on are not seen by all rows
-      const int region = max(p.mask != nullptr ? r.prefix : r.prefix + first + 1, 0);
+    for (;; ++piece) {
+      // what a piece is stays in shared memory, so as not to take registers
+      // through the tile loop
+      const TreePiece& pc = sm.piece[piece % kPieceRing];
+      ok = __all_sync(0xffffffffu,
+                      wait(&sm.piece_full[piece % kPieceRing], piece / kPieceRing & 1));
+      if (!ok || pc.end) break;
+      const int t0 = pc.t0, t1 = pc.t1;
+      const int region = pc.region;
       float m = -INFINITY, l = 0.0f;
       const int step = DUAL ? 1 : 2;
       bool fresh = true;
@@ -718,10 +746,22 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         ++tiles_done;
         tc_fence_after();
         const uint4 words = *reinterpret_cast<const uint4*>(sm.meta[seq % kMetaRing]);
-        uint32_t w[4] = {words.x, words.y, words.z, words.w};
-        const bool masked = (t + 1) * kTile > region || (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu;
+        const bool masked = (t + 1) * kTile > region ||
+                            (words.x & words.y & words.z & words.w) != 0xffffffffu;
         if (masked) {
-          row_mask(w, p, r, t, i, i0, local, R, lane);
+          uint32_t w[4] = {words.x, words.y, words.z, words.w};
+          row_mask(w, p, pc.r, t, pc.first + (DUAL ? st * R : 0), g.group_div.div(row), R, lane);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // hidden scores become -inf in place
+            uint32_t s[32];
+            tmem_ld32(ts + k * 32, s);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((w[k] >> e) & 1)) s[e] = 0xff800000u;
+            tmem_st32(ts + k * 32, s);
+          }
+          tmem_wait_st();
           // Values of tokens that may not be read become 0; infinite or NaN
           // elements of drafted tokens too, and the piece remembers them.
           const int vseq = 2 * seq + 1;
@@ -772,19 +812,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         uint32_t pk[kTile / 2];
         float2 sum;
         for (bool settled = false;;) {
-          const float shift = m == -INFINITY ? 0.0f : -m * c;
-          float high = -INFINITY;
-          sum = make_float2(0.0f, 0.0f);
-          uint32_t sr[2][32];
-          tmem_ld32(ts, sr[0]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            tmem_wait_ld();
-            if (k < 3) tmem_ld32(ts + (k + 1) * 32, sr[(k + 1) & 1]);
-            if (masked) hide32(sr[k & 1], w[k]);
-            high = fmaxf(high, max32(sr[k & 1]));
-            exp_pairs<F16>(sr[k & 1], pk + k * 16, c, shift, sum);
-          }
+          const float high = score_pass<F16>(ts, c, m, pk, sum);
           if (settled) break;
           const bool move =
               fresh || (high > m && (m == -INFINITY || (high - m) * c > kSlack));
@@ -812,7 +840,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         l += sum.x + sum.y;
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&sm.p_ready[st]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_ready[st]);
       }
       if (!ok) break;
       // ---- the piece's end: sums, outputs or partials
@@ -841,11 +870,16 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
       }
       if (DUAL || st == 0) {
         tc_fence_after();
-        const bool whole = tiles == u.tiles;
+        const TreeRequest r = pc.r;
+        int local, head;
+        g.group_div.divmod(row, local, head);
+        const int i = pc.first + (DUAL ? st * R : 0) + local;  // this thread's row of the request
+        const bool live = local < R && i < r.count;
+        const bool whole = tiles == pc.tiles;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const float lse2 = l == 0.0f ? -INFINITY : m * c + log2f(l);
         const int64_t packed = r.row0 + i;
-        const int q_head = u.h * p.group + head;
+        const int q_head = pc.h * p.group + head;
         const int64_t part_row =
             (static_cast<int64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * C::kRows +
             (DUAL ? st * kTile : 0) + row;
@@ -878,11 +912,11 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
               if (!tree_sees(p, r, i, t)) continue;
               int q, at;
               p.page_div.divmod(t, q, at);
-              const int page = p.table[u.b * p.table_stride + q];
+              const int page = p.table[pc.b * p.table_stride + q];
               if (page < 0 || page >= p.num_blocks) continue;
               const uint16_t* v = static_cast<const uint16_t*>(p.v_cache) +
                                   page * p.v_block_stride + at * p.v_token_stride +
-                                  u.h * p.v_head_stride + k;
+                                  pc.h * p.v_head_stride + k;
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
                 const float x = unpack<F16>(v[e]);
@@ -926,7 +960,6 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         if (!DUAL) mbar_arrive(&sm.xchg[1]);  // O of both is free
       }
       n += tiles;
-      if (!unit_next(p, u, span)) break;
     }
     if (!ok && lane == 0) give_up();
     __syncwarp();
