@@ -25,7 +25,7 @@ BUILD = ROOT / "_build"
 LIB = PKG / "libqsa_b200.so"
 SOURCES = ["capi.cu", "topk.cu", "indexer.cu", "indexer_tc.cu", "select_decode.cu", "attention.cu",
            "static_scratch.cu", "prepare.cu", "rotary.cu", "tree_attention.cu",
-           "tree_attention_tc.cu", "cache_move.cu",
+           "tree_attention_tc.cu", "attention_weights_tc.cu", "cache_move.cu",
            "selftest.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler",

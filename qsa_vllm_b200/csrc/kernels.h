@@ -377,6 +377,9 @@ bool tree_attention_tc_eligible(const TreeParams& p);
 cudaError_t launch_tree_attention_tc(const TreeParams& p, cudaStream_t stream);
 size_t tree_attention_tc_workspace(int group, int dim, int max_query_len);
 cudaError_t launch_attention_weights(const TreeParams& p, cudaStream_t stream);
+// tcgen05 + TMA form (attention_weights_tc.cu), dispatched likewise.
+bool attention_weights_tc_eligible(const TreeParams& p);
+cudaError_t launch_attention_weights_tc(const TreeParams& p, cudaStream_t stream);
 
 int num_sms();
 // One CTA waits on an mbarrier phase nothing completes; the bounded wait

@@ -257,6 +257,10 @@ cudaError_t launch_attention_weights(const TreeParams& p, cudaStream_t stream) {
   const int tokens = static_cast<int>(std::min<int64_t>(reach, p.capacity));
   const int tiles = (tokens + kGenThreads - 1) / kGenThreads;
   if (tiles == 0) return cudaSuccess;
+  if (attention_weights_tc_eligible(p)) {
+    const cudaError_t e = launch_attention_weights_tc(p, stream);
+    if (e != cudaErrorNotSupported) return e;
+  }
   return count_launches(launch_kernel(attention_weights_general,
                                       dim3(tiles, p.requests * p.kv_heads), dim3(kGenThreads), 0,
                                       stream, 1, p));

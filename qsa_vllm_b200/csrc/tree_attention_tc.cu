@@ -207,15 +207,6 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t saddr) {
   return d;
 }
 
-// One lane of a converged warp.
-__device__ __forceinline__ bool elect_lane() {
-  uint32_t yes;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(yes));
-  return yes != 0;
-}
-
 // A place in the ring of key and value tiles, which alternate.
 struct RingPos {
   int slot;
@@ -240,52 +231,6 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
       : "memory");
 }
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1,
-                                            int c2, int c3, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive_expect(uint64_t* bar, uint32_t bytes) {
-  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::
-                   "r"(smem_u32(bar)),
-               "r"(bytes)
-               : "memory");
-}
-
-#define QSA_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), \
-                     "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
-#define QSA_I8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), \
-                     "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
-// 32 columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : QSA_R8(r, 0), QSA_R8(r, 8), QSA_R8(r, 16), QSA_R8(r, 24)
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-      "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::
-          QSA_I8(r, 0),
-      QSA_I8(r, 8), QSA_I8(r, 16), QSA_I8(r, 24), "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (F16) {
@@ -302,31 +247,6 @@ __device__ __forceinline__ float unpack(uint16_t x) {
 }
 
 // ------------------------------------------------------------------ softmax
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
-      "%13,%14,%15};" ::QSA_I8(r, 0),
-      QSA_I8(r, 8), "r"(taddr)
-      : "memory");
-}
-
-// Two 32-bit operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
-        "l"(*reinterpret_cast<uint64_t*>(&c)));
-  return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -1059,24 +979,6 @@ void tree_shape(int group, int max_query_len, bool* dual, int* cohort) {
   *cohort = std::min(units, 4);
 }
 
-bool encode_rows(CUtensorMap* map, bool f16, const void* base, const cuuint64_t (&dims)[4],
-                 const int64_t (&strides)[3], const cuuint32_t (&box)[4]) {
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  cuuint64_t bytes[3];
-  for (int i = 0; i < 3; ++i) {
-    // the stride of a dimension of size 1 is never used, but is checked
-    bytes[i] = static_cast<cuuint64_t>(dims[i + 1] == 1 ? 64 : strides[i]) * 2;
-    if (dims[i + 1] > 1 && (strides[i] <= 0 || bytes[i] % 16 != 0)) return false;
-  }
-  return tensor_map_encoder()(map,
-                              f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                              4, const_cast<void*>(base), dims, bytes, box, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, bool DUAL, bool F16>
 cudaError_t launch_tree_typed(const TreeParams& p, TreeGeometry& g, const CUtensorMap& qmap,
                               const CUtensorMap& kmap, const CUtensorMap& vmap,
@@ -1105,6 +1007,24 @@ cudaError_t launch_tree_rows(bool dual, const TreeParams& p, TreeGeometry& g,
 }
 
 }  // namespace
+
+bool encode_rows(CUtensorMap* map, bool f16, const void* base, const cuuint64_t (&dims)[4],
+                 const int64_t (&strides)[3], const cuuint32_t (&box)[4]) {
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  cuuint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    // the stride of a dimension of size 1 is never used, but is checked
+    bytes[i] = static_cast<cuuint64_t>(dims[i + 1] == 1 ? 64 : strides[i]) * 2;
+    if (dims[i + 1] > 1 && (strides[i] <= 0 || bytes[i] % 16 != 0)) return false;
+  }
+  return tensor_map_encoder()(map,
+                              f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                              4, const_cast<void*>(base), dims, bytes, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 size_t tree_attention_tc_workspace(int group, int dim, int max_query_len) {
   if ((dim != 64 && dim != 128) || group > kTile) return 0;
