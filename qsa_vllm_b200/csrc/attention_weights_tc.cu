@@ -40,6 +40,7 @@ constexpr int kTile = 128;     // tokens per tile
 constexpr int kPairs = 256;    // (row, head) pairs of one pass
 constexpr int kPieceRing = 4;
 constexpr int kWTmemCols = 512;
+constexpr int kBuffers = 4;    // of 128 columns; passes of more pairs take two at a time
 
 template <int D>
 struct WeightsCfg {
@@ -61,21 +62,24 @@ struct WeightsSmem {
   using C = WeightsCfg<D>;
   alignas(1024) uint8_t ring[C::S][C::kTileBytes];
   alignas(1024) uint8_t q[C::kSub][C::kQSubBytes];
-  float4 pair[kPairs / 2];  // of two pairs: (-lse2, -lse2, factor, factor)
-  int row[kPairs];          // the request's row of a pair
+  float shift[kPairs];      // of a pair: -lse2 (+ log2 of a factor above 0)
+  float factor[kPairs];     // what is left of the factor
   int list[kPairs];         // rows that count, of this pass
-  uint64_t full[C::S], empty[C::S], s_full[2], s_empty[2], q_ready, drain;
+  uint64_t full[C::S], empty[C::S], s_full[kBuffers], s_empty[kBuffers], q_ready, drain;
   uint64_t piece_full[kPieceRing], piece_empty[kPieceRing], sync, taken;
   WeightsPiece piece[kPieceRing];
   int64_t scan[kWThreads / 32], first_base;
   int first_b;
   int pairs;        // of this pass
+  uint32_t bits[kPairs][4];  // first 128 drafted tokens that a listed row sees
+  int folded[8];    // per epilogue warp: its factors all went into the shifts
   int next_row;     // where the next pass goes on; r.count when there is none
   uint32_t tmem_base;
   int abort_flag;
 };
 
 struct WeightsGeometry {
+  FastDiv group_div;
   int box_rows;
   int ranges;
 };
@@ -85,6 +89,11 @@ __device__ __forceinline__ int weight_tokens(const TreeParams& p, const TreeRequ
 }
 __device__ __forceinline__ int weight_tiles(const TreeParams& p, int b) {
   return (weight_tokens(p, tree_request_info(p, b)) + kTile - 1) / kTile;
+}
+
+// TMEM buffer of the j-th tile of a pass.
+__device__ __forceinline__ int weights_buffer(int j, int pairs) {
+  return pairs <= 128 ? j & 3 : (j & 1) * 2;
 }
 
 template <int D, bool F16>
@@ -103,7 +112,7 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kBuffers; ++s) {
       mbar_init(&sm.s_full[s], 1);
       mbar_init(&sm.s_empty[s], 4);
     }
@@ -274,6 +283,7 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
     const uint64_t q_desc = sw128_desc(smem_u32(sm.q[0]));
     const uint64_t k_desc = sw128_desc(smem_u32(sm.ring[0]));
     int seq = 0, passes = 0;
+    uint32_t freed = 0;  // phase of each buffer's s_empty
     for (int piece = 0;; ++piece) {
       const WeightsPiece& pc = sm.piece[piece % kPieceRing];
       ok = arrived(&sm.piece_full[piece % kPieceRing], piece / kPieceRing & 1);
@@ -293,16 +303,17 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
         const uint32_t idesc =
             (1u << 4) | (fmt << 7) | (fmt << 10) | ((n16 * 2) << 17) | ((kTile >> 4) << 24);
         for (int j = 0; j < m; ++j, ++seq) {
-          const int slot = seq % C::S, a = seq & 1;
+          const int slot = seq % C::S, a = weights_buffer(j, pairs);
           ok = arrived(&sm.full[slot], (seq / C::S) & 1) &&
-               arrived(&sm.s_empty[a], ((seq >> 1) & 1) ^ 1);
+               arrived(&sm.s_empty[a], ((freed >> a) & 1) ^ 1);
           if (!ok) break;
+          freed ^= 1u << a;
           tc_fence_after();
           if (leader) {
             const uint64_t ka = k_desc + static_cast<uint32_t>(slot) * (C::kTileBytes >> 4);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              umma_bf16(tmem + a * 256, ka + (((k / 4) * C::kSubBytes + (k % 4) * 32) >> 4),
+              umma_bf16(tmem + a * 128, ka + (((k / 4) * C::kSubBytes + (k % 4) * 32) >> 4),
                         q_desc + (((k / 4) * C::kQSubBytes + (k % 4) * 32) >> 4), idesc, k > 0);
             umma_commit(&sm.empty[slot]);
             umma_commit(&sm.s_full[a]);
@@ -325,11 +336,11 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
     const int st = warp >= 6 ? 1 : 0;
     const int quad = warp & 3, token = quad * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t ts = tmem + st * 256 + lane_off;
     const float c = p.scale_log2;
     const float2 c2 = make_float2(c, c);
     const int rows_per_pass = kPairs / p.group;
-    int seq = 0, syncs = 0, passes = 0;
+    int syncs = 0, passes = 0;
+    uint32_t filled = 0;  // phase of each buffer's s_full
     // all eight warps meet
     auto meet = [&]() -> bool {
       __syncwarp();
@@ -388,7 +399,8 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
           const int n = x / (D / 8), ch = x - n * (D / 8);
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
           if (n < pairs) {
-            const int j = n / p.group, head = n - j * p.group;
+            int j, head;
+            g.group_div.divmod(n, j, head);
             v = *reinterpret_cast<const uint4*>(
                 static_cast<const uint16_t*>(p.q) +
                 static_cast<int64_t>(r.row0 + sm.list[j]) * p.q_row_stride +
@@ -396,7 +408,23 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
           }
           *reinterpret_cast<uint4*>(sm.q[ch / 8] + n * 128 + (((ch % 8) ^ (n % 8)) * 16)) = v;
         }
-        if (et < (pairs + 31) / 32 * 32) {
+        if (p.mask != nullptr && pc.t1 * kTile > r.prefix) {
+          const int listed = g.group_div.div(pairs);
+          for (int x = warp - 2; x < listed; x += 8) {
+            const uint8_t* bytes = p.mask + (r.row0 + sm.list[x]) * p.mask_stride;
+            uint8_t byte[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              byte[k] = k * 32 + lane < p.mask_width ? bytes[k * 32 + lane] : 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t word = __ballot_sync(0xffffffffu, byte[k] != 0);
+              if (lane == 0) sm.bits[x][k] = word;
+            }
+          }
+        }
+        bool fold = true;
+        {
           float l = 0.0f, f = 0.0f;
           int i = -1;
           if (et < pairs) {
@@ -405,83 +433,135 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
             const int64_t row = r.row0 + i;
             l = p.lse[row * p.lse_row_stride + pc.h * p.group + head] * -1.4426950408889634f;
             f = p.row_factors == nullptr ? 1.0f : p.row_factors[row * p.factor_stride];
+            if (l == INFINITY) l = -INFINITY;  // a head that saw nothing
+            fold = f > 0.0f && f < INFINITY && l == l;
+            if (fold) {
+              l += log2f(f);
+              f = 1.0f;
+            }
+          } else {
+            l = -INFINITY;  // columns of no pair add nothing
           }
-          float* out = reinterpret_cast<float*>(&sm.pair[et / 2]) + (et & 1);
-          out[0] = l;
-          out[2] = f;
-          sm.row[et] = i;
+          sm.shift[et] = l;
+          sm.factor[et] = f;
         }
+        fold = __all_sync(0xffffffffu, fold);
+        if (lane == 0) sm.folded[warp - 2] = fold;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.q_ready);
         // sums of a pass read what all warps wrote
         ok = meet();
         if (!ok) break;
+        int folds = 1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) folds &= sm.folded[k];  // also no NaN among the log-sum-exps
+        // The weight so far and the page of this thread's token in a tile are
+        // fetched a tile ahead, the weight into L2 kAhead tiles before that:
+        // behind the key tiles in flight memory takes longer than two tiles.
+        constexpr int kAhead = 4;
+        auto prefetch = [&](int j) {
+          const int tok = (t0 + j) * kTile + token;
+          if (j < m && tok < tokens && (lane & 7) == 0)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"((first ? w_in : w_out) + tok));
+        };
+        auto fetch = [&](int j, float& was, int& page) {
+          const int tok = (t0 + j) * kTile + token;
+          was = 0.0f;
+          page = -1;
+          prefetch(j + kAhead);
+          if (j >= m || tok >= tokens) return;
+          was = first ? w_in[tok] : w_out[tok];
+          int q, at;
+          p.page_div.divmod(tok, q, at);
+          page = ld_once(table + q);
+        };
+        for (int j = st; j < st + kAhead; j += 2) prefetch(j);
+        float was_next;
+        int page_next;
+        fetch(st, was_next, page_next);
         for (int j = 0; j < m; ++j) {
           const int t = t0 + j, tok = t * kTile + token;
-          if (pairs > 0) {
-            if (((seq + j) & 1) != st) continue;
-          } else if ((j & 1) != st) {
-            continue;
-          }
+          const int a = weights_buffer(j, pairs);
+          const uint32_t phase = (filled >> a) & 1;
+          if (pairs > 0) filled ^= 1u << a;  // the other warpgroup's buffers too
+          if ((j & 1) != st) continue;
           const bool here = tok < tokens;
-          float was = 0.0f;
-          if (here) was = first ? w_in[tok] : w_out[tok];
+          const float was = was_next;
+          const int page = page_next;
           float got = 0.0f;
+          fetch(j + 2, was_next, page_next);
           if (pairs > 0) {
-            ok = arrived(&sm.s_full[st], ((seq + j) >> 1) & 1);
+            ok = arrived(&sm.s_full[a], phase);
             if (!ok) break;
             tc_fence_after();
-            int q, at;
-            p.page_div.divmod(here ? tok : 0, q, at);
-            const int page = here ? ld_once(table + q) : -1;
-            const bool exists = page >= 0 && page < p.num_blocks;
             const bool drafted = (t + 1) * kTile > r.prefix;  // some tokens not seen by all
+            const uint32_t ts = tmem + a * 128 + lane_off;
             float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll 1
             for (int k = 0; k < pairs; k += 32) {
               uint32_t v[32];
               tmem_ld32(ts + k, v);
-              tmem_wait_ld();
+              uint32_t sees = pairs - k >= 32 ? 0xffffffffu : (1u << (pairs - k)) - 1;
               if (drafted) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const int i = sm.row[k + e];
-                  if (i < 0 || !here || !tree_sees(p, r, i, tok)) continue;
-                  const float* pr = reinterpret_cast<const float*>(&sm.pair[(k + e) / 2]) + (e & 1);
-                  acc[0].x = fmaf(pr[2], fast_exp2(fmaf(__uint_as_float(v[e]), c, pr[0])),
-                                  acc[0].x);
+                // each row's bit once, then spread over its heads' columns
+                uint32_t rows = 0, cols = 0;
+                const int j0 = k / p.group, j1 = (min(k + 32, pairs) - 1) / p.group;
+#pragma unroll 4
+                for (int x = j0; x <= j1; ++x) {
+                  const int node = tok - r.prefix;
+                  bool see;
+                  if (p.mask == nullptr || node >= kTile) see = tree_sees(p, r, sm.list[x], tok);
+                  else see = node < 0 || ((sm.bits[x][node >> 5] >> (node & 31)) & 1);
+                  rows |= static_cast<uint32_t>(here && see) << (x - j0);
                 }
-              } else if (k + 32 > pairs) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  if (k + e >= pairs) break;
-                  const float* pr = reinterpret_cast<const float*>(&sm.pair[(k + e) / 2]) + (e & 1);
-                  acc[e & 1].x = fmaf(pr[2], fast_exp2(fmaf(__uint_as_float(v[e]), c, pr[0])),
-                                      acc[e & 1].x);
+                for (int e = 0; e < 32; ++e)
+                  cols |= ((rows >> ((g.group_div.div(k + e) - j0) & 31)) & 1) << e;
+                sees &= cols;
+              }
+              tmem_wait_ld();
+              if (folds) {
+                // a hidden score becomes -inf, and its exponential 0
+                if (sees != 0xffffffffu) {
+#pragma unroll
+                  for (int e = 0; e < 32; ++e)
+                    if (!((sees >> e) & 1)) v[e] = 0xff800000u;
                 }
-              } else {
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                  const float4 pr = sm.pair[(k + e) / 2];
+                for (int e = 0; e < 32; e += 4) {
+                  const float4 sh = *reinterpret_cast<const float4*>(&sm.shift[k + e]);
                   float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2,
-                                  make_float2(pr.x, pr.y));
+                                  make_float2(sh.x, sh.y));
+                  float2 y = fma2(make_float2(__uint_as_float(v[e + 2]),
+                                              __uint_as_float(v[e + 3])), c2,
+                                  make_float2(sh.z, sh.w));
                   x.x = fast_exp2(x.x);
                   x.y = fast_exp2(x.y);
-                  acc[e / 2 & 1] = fma2(x, make_float2(pr.z, pr.w), acc[e / 2 & 1]);
+                  y.x = fast_exp2(y.x);
+                  y.y = fast_exp2(y.y);
+                  acc[0] = add2(acc[0], x);
+                  acc[1] = add2(acc[1], y);
+                }
+              } else {  // a factor below 0, infinite or NaN, or a NaN log-sum-exp
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float x =
+                      sm.factor[k + e] *
+                      fast_exp2(fmaf(__uint_as_float(v[e]), c, sm.shift[k + e]));
+                  acc[e & 1].x += (sees >> e) & 1 ? x : 0.0f;
                 }
               }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.s_empty[st]);
+            if (lane == 0) mbar_arrive(&sm.s_empty[a]);
             acc[0] = add2(acc[0], acc[1]);
-            if (exists) got = acc[0].x + acc[0].y;
+            if (page >= 0 && page < p.num_blocks) got = acc[0].x + acc[0].y;
           }
           if (here) w_out[tok] = was + got;
         }
         if (!ok) break;
-        if (pairs > 0) seq += m;
         // the next pass writes the queries over: every product of this one is
         // behind its scores, which both warpgroups have read
         ok = arrived(&sm.taken, passes++ & 1) && meet();
@@ -528,6 +608,7 @@ cudaError_t launch_attention_weights_tc(const TreeParams& p, cudaStream_t stream
   WeightsGeometry g = {};
   g.box_rows = gcd_int(p.page_size, kTile);
   g.ranges = num_sms();
+  g.group_div = FastDiv(static_cast<uint32_t>(p.group));
   const bool f16 = p.dtype == kDtypeF16;
   CUtensorMap kmap;
   if (!encode_rows(&kmap, f16, p.k_cache,

@@ -363,9 +363,10 @@ __device__ __forceinline__ TreeRequest tree_request_info(const TreeParams& p, in
 // Whether packed row `row`, the request's row i, sees token t < r.tokens.
 __device__ __forceinline__ bool tree_sees(const TreeParams& p, const TreeRequest& r, int i, int t) {
   const int node = t - r.prefix;
-  if (node < 0) return true;
   if (p.mask == nullptr) return node <= i;
-  return node < p.mask_width && p.mask[(r.row0 + i) * p.mask_stride + node] != 0;
+  const bool drafted = node >= 0 && node < p.mask_width;
+  const uint8_t bit = drafted ? p.mask[(r.row0 + i) * p.mask_stride + node] : 0;
+  return node < 0 || bit != 0;
 }
 cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t stream);
 size_t tree_attention_workspace(int rows, int requests, int q_heads, int kv_heads, int dim,
