@@ -592,7 +592,15 @@ cudaError_t launch_topk(const TopkParams& p0, cudaStream_t stream, int* plan_clu
   // Smallest (keys per thread, cluster width) whose slices cover the row.
   int V = 8;
   int C = pow2_ceil((w + kThreads * V - 1) / (kThreads * V));
-  if (C > kMaxCluster) {
+  // Eight keys per thread finish a row soonest, as long as all rows' clusters
+  // run at once.  A CTA has its SM to itself, and a cluster lies within one
+  // group of SMs, so about 37 clusters of 4 run at once, 12 of 8 and 4 of 16;
+  // with more rows than that, 32 keys per thread in a quarter of the CTAs win
+  // (us, 8 against 32 keys: 32768 columns 32 rows 15 / 22, 64 rows 30 / 21;
+  // 65536 columns 8 rows 23 / 26, 16 rows 40 / 22; 131072 columns 4 rows
+  // 44 / 25, 32 rows 214 / 30).
+  const int at_once = C <= 4 ? num_sms() / 4 : C == 8 ? num_sms() / 12 : 0;
+  if (C > kMaxCluster || (C >= 4 && p.rows > at_once)) {
     V = 32;
     C = pow2_ceil((w + kThreads * V - 1) / (kThreads * V));
   }
