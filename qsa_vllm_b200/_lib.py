@@ -145,11 +145,22 @@ class _Here:
 _HERE = _Here()
 
 
-def on_device(device: torch.device):
-    """``torch.cuda.device(device)``, free of charge when it is the current one already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+def on_device(index: int):
+    """``torch.cuda.device(index)``, free of charge when it is the current one already."""
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def ready(t: torch.Tensor) -> int:
+    """Index of the tensor's device, checked like :func:`ensure_device` (once per device)."""
+    index = t.get_device()
+    if index not in _checked_devices:
+        ensure_device(t.device)
+    return index
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of a device that is in use, as ``stream_ptr`` without its objects."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -244,9 +244,9 @@ struct RotaryParams {
   int interleaved, inverse, dtype;
   int vec;                 // 16-byte chunks everywhere
   int q_in_place, k_in_place;
-  // filled by launch_rotary: items of one token, and their division into heads
-  int q_items, k_items;
-  FastDiv item_div, q_head_div, k_head_div, v_head_div;
+  // filled by launch_rotary
+  int heads_at_once, parts;
+  FastDiv chunk_div, rest_div, value_div, part_div;
   int* err;
 };
 cudaError_t launch_rotary(RotaryParams p, cudaStream_t stream);

@@ -21,42 +21,49 @@ import torch
 
 from . import _lib
 from .qsa import aligned_head_rows
-from .tree_attention import check_tree_arguments, mask_arguments
+from .tree_attention import check_lse, check_tree_arguments, mask_arguments
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.dim() != 4 or c.shape != k_cache.shape:
-            raise ValueError(f"{what}: {name} must be [blocks, page, kv_heads, dim], both alike")
-        if c.dtype not in _DTYPES or c.dtype != k_cache.dtype:
-            raise TypeError(f"{what}: {name} must be bfloat16, float16 or float32, both alike")
-        if c.device != k_cache.device:
-            raise TypeError(f"{what}: {name} must be on {k_cache.device}")
-        if c.stride(3) != 1 and c.shape[3] > 1:
-            raise ValueError(f"{what}: {name} needs a unit head-dim stride")
+def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple:
+    """The arguments that describe two caches, once they are found in order."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError(f"{what}: the caches must be [blocks, page, kv_heads, dim], both alike")
+    kind = _DTYPES.get(k_cache.dtype)
+    if kind is None or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"{what}: the caches must be bfloat16, float16 or float32, both alike")
+    if v_cache.get_device() != k_cache.get_device():
+        raise TypeError(f"{what}: v_cache must be on {k_cache.device}")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if (ks[3] != 1 or vs[3] != 1) and shape[3] > 1:
+        raise ValueError(f"{what}: the caches need a unit head-dim stride")
+    return (k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+            shape[0], shape[1], shape[2], shape[3], kind)
 
 
-def _int32(what: str, name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> None:
+def _int32(what: str, name: str, t: torch.Tensor, dev: int, *shape) -> None:
     """int32 of this shape (None: any size), with unit stride over its last dim."""
-    if t.dtype != torch.int32 or t.device != device:
-        raise TypeError(f"{what}: {name} must be int32 on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    if t.dtype != torch.int32 or t.get_device() != dev:
+        raise TypeError(f"{what}: {name} must be int32 on the caches' device, got {t.dtype} on "
+                        f"{t.device}")
+    got = t.shape
+    if len(got) != len(shape) or any([n is not None and n != m for n, m in zip(shape, got)]):
         want = tuple("any" if n is None else n for n in shape)
-        raise ValueError(f"{what}: {name} must be {want}, got {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: {name} must be {want}, got {tuple(got)}")
+    if got[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: {name} needs a unit stride over its last dim")
 
 
-def _cache_args(k_cache, v_cache, block_table, out_table) -> tuple:
-    out = (None, 0, 0) if out_table is None else (out_table.data_ptr(), out_table.stride(0),
-                                                  out_table.shape[1])
-    return (k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-            v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
-            k_cache.shape[0], k_cache.shape[1], k_cache.shape[2], k_cache.shape[3],
-            _DTYPES[k_cache.dtype], block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[1], *out)
+def _tables(what: str, dev: int, block_table: torch.Tensor, out_table) -> tuple:
+    _int32(what, "block_table", block_table, dev, None, None)
+    requests, width = block_table.shape
+    if out_table is None:
+        return block_table.data_ptr(), block_table.stride(0), width, None, 0, 0
+    _int32(what, "out_table", out_table, dev, requests, None)
+    return (block_table.data_ptr(), block_table.stride(0), width, out_table.data_ptr(),
+            out_table.stride(0), out_table.shape[1])
 
 
 def accumulate_attention_weights(
@@ -76,42 +83,44 @@ def accumulate_attention_weights(
     max_query_len = int(max_query_len)
     check_tree_arguments(what, q, (("k_cache", k_cache),), block_table, seq_lens,
                          query_start_loc, tree_mask, max_query_len)
-    dev = q.device
     rows, hq, d = q.shape
-    requests, hkv = block_table.shape[0], k_cache.shape[2]
+    requests, width = block_table.shape
+    blocks, page, hkv, _ = k_cache.shape
+    dev = q.get_device()
     if out is None:
         out = weights
-    for name, w in (("weights", weights), ("out", out)):
-        if w.dtype != torch.float32 or w.device != dev:
-            raise TypeError(f"{what}: {name} must be float32 on {dev}")
-        if w.dim() != 3 or w.shape[:2] != (requests, hkv) or w.shape != weights.shape \
-                or (w.shape[2] > 1 and w.stride(2) != 1):
-            raise ValueError(f"{what}: {name} must be [{requests}, {hkv}, capacity] with a unit "
-                             "token stride")
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or lse.device != dev \
-            or (lse.stride(1) != 1 and hq > 1):
-        raise ValueError(f"{what}: lse must be float32 [rows, heads] with a unit head stride")
-    if row_factors is not None and (row_factors.dtype != torch.float32
-                                    or row_factors.shape != q.shape[:1]
-                                    or row_factors.device != dev):
+    shape = weights.shape
+    if len(shape) != 3 or shape[0] != requests or shape[1] != hkv or out.shape != shape:
+        raise ValueError(f"{what}: weights and out must be [{requests}, {hkv}, capacity]")
+    ws, os = weights.stride(), out.stride()
+    if weights.dtype != torch.float32 or out.dtype != torch.float32 \
+            or weights.get_device() != dev or out.get_device() != dev:
+        raise TypeError(f"{what}: weights and out must be float32 on {q.device}")
+    if (ws[2] != 1 or os[2] != 1) and shape[2] > 1:
+        raise ValueError(f"{what}: weights and out need a unit token stride")
+    check_lse(what, lse, q)
+    if row_factors is not None and (row_factors.dtype != torch.float32 or row_factors.dim() != 1
+                                    or row_factors.shape[0] != rows
+                                    or row_factors.get_device() != dev):
         raise ValueError(f"{what}: row_factors must be float32 [rows]")
-    _lib.ensure_device(dev)
+    _lib.ready(q)
     if rows:
         q = aligned_head_rows(q)
+    qs, ks = q.stride(), k_cache.stride()
     with _lib.on_device(dev):
-        _lib.check(_lib.load_library().qsa_attention_weights(
-            q.data_ptr(), q.stride(0), q.stride(1), rows, hq, d, _DTYPES[q.dtype],
-            k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-            k_cache.shape[0], k_cache.shape[1], hkv,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], requests,
+        status = _lib.load_library().qsa_attention_weights(
+            q.data_ptr(), qs[0], qs[1], rows, hq, d, _DTYPES[q.dtype],
+            k_cache.data_ptr(), ks[0], ks[1], ks[2], blocks, page, hkv,
+            block_table.data_ptr(), block_table.stride(0), width, requests,
             seq_lens.data_ptr(), query_start_loc.data_ptr(),
             *mask_arguments(tree_mask, seq_lens), max_query_len,
-            d ** -0.5 if scale is None else float(scale), lse.data_ptr(), lse.stride(0),
+            d ** -0.5 if scale is None else scale, lse.data_ptr(), lse.stride(0),
             None if row_factors is None else row_factors.data_ptr(),
             0 if row_factors is None else row_factors.stride(0),
-            weights.data_ptr(), weights.stride(0), weights.stride(1),
-            out.data_ptr(), out.stride(0), out.stride(1), weights.shape[2],
-            _lib.stream_ptr(dev)), what)
+            weights.data_ptr(), ws[0], ws[1], out.data_ptr(), os[0], os[1], shape[2],
+            _lib.raw_stream(dev))
+    if status:
+        _lib.check(status, what)
     return out
 
 
@@ -127,26 +136,26 @@ def cache_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: tor
     read.  Entries outside the tables or on unmapped pages are skipped and set the device error
     word."""
     what = "cache_compact"
-    _caches(what, k_cache, v_cache)
-    dev = k_cache.device
+    caches = _caches(what, k_cache, v_cache)
+    dev = k_cache.get_device()
+    tables = _tables(what, dev, block_table, out_table)
     requests = block_table.shape[0]
-    _int32(what, "block_table", block_table, (None, None), dev)
     if indices.dim() == 3:
-        _int32(what, "indices", indices, (requests, k_cache.shape[2], None), dev)
+        _int32(what, "indices", indices, dev, requests, caches[10], None)
         head_stride = indices.stride(1)
     else:
-        _int32(what, "indices", indices, (requests, None), dev)
+        _int32(what, "indices", indices, dev, requests, None)
         head_stride = 0
     if starts is not None:
-        _int32(what, "starts", starts, (requests,), dev)
-    if out_table is not None:
-        _int32(what, "out_table", out_table, (requests, None), dev)
-    _lib.ensure_device(dev)
+        _int32(what, "starts", starts, dev, requests)
+    _lib.ready(k_cache)
     with _lib.on_device(dev):
-        _lib.check(_lib.load_library().qsa_cache_compact(
-            *_cache_args(k_cache, v_cache, block_table, out_table), requests,
-            indices.data_ptr(), indices.stride(0), head_stride, indices.shape[-1],
-            None if starts is None else starts.data_ptr(), _lib.stream_ptr(dev)), what)
+        status = _lib.load_library().qsa_cache_compact(
+            *caches, *tables, requests, indices.data_ptr(), indices.stride(0), head_stride,
+            indices.shape[-1], None if starts is None else starts.data_ptr(),
+            _lib.raw_stream(dev))
+    if status:
+        _lib.check(status, what)
 
 
 def cache_evict_workspace_bytes(requests: int, list_heads: int, budget: int, sinks: int,
@@ -171,46 +180,48 @@ def cache_evict(weights: torch.Tensor, seq_lens: torch.Tensor, block_table: torc
     length.  kept: int32 ``[B, heads of weights, budget]``, the old token numbers, -1 behind the
     last; lengths: int32 ``[B]``."""
     what = "cache_evict"
-    _caches(what, k_cache, v_cache)
-    dev = k_cache.device
-    requests, heads = block_table.shape[0], k_cache.shape[2]
-    _int32(what, "block_table", block_table, (None, None), dev)
-    _int32(what, "seq_lens", seq_lens, (requests,), dev)
-    if out_table is not None:
-        _int32(what, "out_table", out_table, (requests, None), dev)
+    caches = _caches(what, k_cache, v_cache)
+    dev = k_cache.get_device()
+    tables = _tables(what, dev, block_table, out_table)
+    requests, heads = block_table.shape[0], caches[10]
+    _int32(what, "seq_lens", seq_lens, dev, requests)
     if weights_out is None:
         weights_out = weights
-    for name, w in (("weights", weights), ("weights_out", weights_out)):
-        if w.dtype != torch.float32 or w.device != dev:
-            raise TypeError(f"{what}: {name} must be float32 on {dev}")
-        if w.dim() != 3 or w.shape[0] != requests or w.shape[1] not in (1, heads) \
-                or w.shape != weights.shape:
-            raise ValueError(f"{what}: {name} must be [{requests}, {heads} or 1, capacity]")
-        if w.shape[2] > 1 and w.stride(2) != 1:
-            raise ValueError(f"{what}: {name} needs a unit token stride")
-    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    shape = weights.shape
+    if len(shape) != 3 or shape[0] != requests or shape[1] not in (1, heads) \
+            or weights_out.shape != shape:
+        raise ValueError(f"{what}: weights and weights_out must be [{requests}, {heads} or 1, "
+                         "capacity]")
+    if weights.dtype != torch.float32 or weights_out.dtype != torch.float32 \
+            or weights.get_device() != dev or weights_out.get_device() != dev:
+        raise TypeError(f"{what}: weights and weights_out must be float32 on {k_cache.device}")
+    ws, os = weights.stride(), weights_out.stride()
+    if (ws[2] != 1 or os[2] != 1) and shape[2] > 1:
+        raise ValueError(f"{what}: weights and weights_out need a unit token stride")
     if sinks < 0 or recent < 0 or budget < sinks + recent:
         raise ValueError(f"{what}: sinks {sinks} + recent {recent} must fit the budget {budget}")
     if kept is None:
-        kept = torch.empty(requests, weights.shape[1], budget, dtype=torch.int32, device=dev)
+        kept = torch.empty(requests, shape[1], budget, dtype=torch.int32, device=k_cache.device)
     else:
-        _int32(what, "kept", kept, (requests, weights.shape[1], budget), dev)
+        _int32(what, "kept", kept, dev, requests, shape[1], budget)
         if not kept.is_contiguous():
             raise ValueError(f"{what}: kept must be contiguous")
-    lengths = torch.empty(requests, dtype=torch.int32, device=dev)
-    _lib.ensure_device(dev)
+    lengths = torch.empty(requests, dtype=torch.int32, device=k_cache.device)
+    _lib.ready(k_cache)
     if not requests:
         return kept, lengths
-    need = cache_evict_workspace_bytes(requests, weights.shape[1], budget, sinks, recent)
+    lib = _lib.load_library()
+    need = lib.qsa_cache_evict_workspace_bytes(requests, shape[1], budget, sinks, recent)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = torch.empty(need, dtype=torch.uint8, device=k_cache.device)
     with _lib.on_device(dev):
-        _lib.check(_lib.load_library().qsa_cache_evict(
-            weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[1],
-            weights.shape[2], seq_lens.data_ptr(), requests, budget, sinks, recent,
-            *_cache_args(k_cache, v_cache, block_table, out_table), weights_out.data_ptr(),
-            weights_out.stride(0), weights_out.stride(1), kept.data_ptr(), lengths.data_ptr(),
-            workspace.data_ptr(), need, _lib.stream_ptr(dev)), what)
+        status = lib.qsa_cache_evict(
+            weights.data_ptr(), ws[0], ws[1], shape[1], shape[2], seq_lens.data_ptr(), requests,
+            budget, sinks, recent, *caches, *tables, weights_out.data_ptr(), os[0], os[1],
+            kept.data_ptr(), lengths.data_ptr(), workspace.data_ptr(), need,
+            _lib.raw_stream(dev))
+    if status:
+        _lib.check(status, what)
     return kept, lengths
 
 

@@ -67,56 +67,46 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str =
 
 
 def _heads(name: str, t: torch.Tensor, like: torch.Tensor, heads: int | None = None) -> None:
-    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] \
-            or (heads is not None and t.shape[1] != heads):
+    """Refuses a tensor that is not [tokens, heads, dim] beside ``like``."""
+    shape, other = t.shape, like.shape
+    if len(shape) != 3 or shape[0] != other[0] or shape[2] != other[2] \
+            or (heads is not None and shape[1] != heads):
         raise ValueError(f"rotary: {name} must be [tokens, heads, dim] matching the others, "
-                         f"got {tuple(t.shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
+                         f"got {tuple(shape)}")
+    if t.dtype != like.dtype or t.get_device() != like.get_device():
         raise TypeError(f"rotary: {name} must be {like.dtype} on {like.device}, "
                         f"got {t.dtype} on {t.device}")
-    if t.stride(2) != 1 and t.shape[2] > 1:
+    if t.stride(2) != 1 and shape[2] > 1:
         raise ValueError(f"rotary: {name} needs a unit head-dim stride")
 
 
-def _call(q, q_out, k, k_out, v, k_cache, v_cache, slots, positions, frequencies, interleaved,
-          inverse, factor) -> None:
-    like = q if q is not None else k
+def _scalars(like: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor) -> None:
+    """Refuses positions and frequencies that do not fit ``like``."""
     if like.dtype not in _DTYPES:
         raise TypeError(f"rotary: bfloat16, float16 or float32 expected, got {like.dtype}")
-    tokens, _, dim = like.shape
-    dev = like.device
-    if positions.dim() != 1 or positions.shape[0] != tokens or positions.dtype != torch.int64:
+    if positions.dim() != 1 or positions.shape[0] != like.shape[0] \
+            or positions.dtype != torch.int64:
         raise ValueError("rotary: positions must be int64 [tokens]")
-    if frequencies.dim() != 1 or frequencies.dtype != torch.float64:
-        raise TypeError("rotary: frequencies must be a float64 vector")
-    rotary_dim = 2 * frequencies.shape[0]
-    if not 2 <= rotary_dim <= dim:
-        raise ValueError(f"rotary: {frequencies.shape[0]} frequencies for a head of {dim}")
-    if positions.device != dev or frequencies.device != dev:
-        raise TypeError(f"rotary: positions and frequencies must be on {dev}")
-    _lib.ensure_device(dev)
-    if tokens == 0:
-        return
-    if not frequencies.is_contiguous():
-        frequencies = frequencies.contiguous()
-    none = (None, 0, 0)
+    if frequencies.dim() != 1 or frequencies.dtype != torch.float64 \
+            or not frequencies.is_contiguous():
+        raise TypeError("rotary: frequencies must be a contiguous float64 vector")
+    if not 2 <= 2 * frequencies.shape[0] <= like.shape[2]:
+        raise ValueError(f"rotary: {frequencies.shape[0]} frequencies for a head of "
+                         f"{like.shape[2]}")
+    if positions.get_device() != like.get_device() \
+            or frequencies.get_device() != like.get_device():
+        raise TypeError(f"rotary: positions and frequencies must be on {like.device}")
 
-    def rows(t):
-        return none if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
 
-    if k_cache is None:
-        caches = (None, 0, 0, 0, None, 0, 0, 0, 0, 0, None, 0)
-    else:
-        caches = (k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                  v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
-                  k_cache.shape[0], k_cache.shape[1], slots.data_ptr(), slots.stride(0))
-    with _lib.on_device(dev):
-        _lib.check(_lib.load_library().qsa_rotary(
-            *rows(q), 0 if q is None else q.shape[1], *rows(q_out),
-            *rows(k), 0 if k is None else k.shape[1], *rows(k_out), *rows(v), *caches,
-            tokens, dim, positions.data_ptr(), positions.stride(0), frequencies.data_ptr(),
-            rotary_dim, factor, 1 if interleaved else 0, 1 if inverse else 0,
-            _DTYPES[like.dtype], _lib.stream_ptr(dev)), "rotary")
+def _side(x: torch.Tensor | None) -> tuple:
+    """Pointer, row and head stride."""
+    if x is None:
+        return None, 0, 0
+    strides = x.stride()
+    return x.data_ptr(), strides[0], strides[1]
+
+
+_NO_CACHE = (None, 0, 0, None, 0, 0, 0, None, 0, 0, 0, 0, 0, None, 0)
 
 
 def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor,
@@ -130,23 +120,40 @@ def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torc
     ``[tokens]``; frequencies: float64 ``[rotary_dim / 2]``.  ``q_out`` / ``k_out`` may be the
     inputs themselves (in place); other overlaps are not allowed.  New contiguous tensors are
     returned where they are None."""
-    if q is None and k is None:
-        raise ValueError("rotary: q or k expected")
     like = q if q is not None else k
-    outs = []
-    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+    if like is None:
+        raise ValueError("rotary: q or k expected")
+    heads = [0, 0]
+    for i, (x, out) in enumerate(((q, q_out), (k, k_out))):
         if x is None:
-            outs.append(None)
             continue
-        _heads(name, x, like)
+        _heads("k" if i else "q", x, like)
+        heads[i] = x.shape[1]
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        else:
-            _heads(name + "_out", out, x, x.shape[1])
-        outs.append(out)
-    _call(q, outs[0], k, outs[1], None, None, None, None, positions, frequencies, interleaved,
-          inverse, float(factor))
-    return outs[0], outs[1]
+            if i:
+                k_out = out
+            else:
+                q_out = out
+        elif out is not x:
+            _heads("k_out" if i else "q_out", out, x, heads[i])
+    if q is None:
+        q_out = None
+    if k is None:
+        k_out = None
+    _scalars(like, positions, frequencies)
+    index = _lib.ready(like)
+    tokens, _, dim = like.shape
+    if tokens:
+        with _lib.on_device(index):
+            status = _lib.load_library().qsa_rotary(
+                *_side(q), heads[0], *_side(q_out), *_side(k), heads[1], *_side(k_out),
+                *_NO_CACHE, tokens, dim, positions.data_ptr(), positions.stride(0),
+                frequencies.data_ptr(), 2 * frequencies.shape[0], factor, interleaved, inverse,
+                _DTYPES[like.dtype], _lib.raw_stream(index))
+        if status:
+            _lib.check(status, "rotary")
+    return q_out, k_out
 
 
 def rotary_store(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -161,29 +168,46 @@ def rotary_store(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     int64 ``[tokens]``, page * page_size + offset.  Tokens with a slot below 0 are not stored;
     one past the cache is not stored either and sets the device error word.  No two tokens may
     share a slot."""
-    like = k
-    _heads("k", k, like)
-    _heads("v", v, like, k.shape[1])
-    for name, c in (("key_cache", key_cache), ("value_cache", value_cache)):
-        if c.dim() != 4 or c.shape[2:] != k.shape[1:] or c.shape != key_cache.shape:
-            raise ValueError(f"rotary: {name} must be [blocks, page, {k.shape[1]}, {k.shape[2]}]")
-        if c.dtype != k.dtype or c.device != k.device:
-            raise TypeError(f"rotary: {name} must be {k.dtype} on {k.device}")
-        if c.stride(3) != 1 and c.shape[3] > 1:
-            raise ValueError(f"rotary: {name} needs a unit head-dim stride")
-    if slots.dim() != 1 or slots.shape[0] != k.shape[0] or slots.dtype != torch.int64 \
-            or slots.device != k.device:
+    _heads("k", k, k)
+    tokens, kv_heads, dim = k.shape
+    _heads("v", v, k, kv_heads)
+    cache, kind, index = key_cache.shape, k.dtype, k.get_device()
+    if len(cache) != 4 or cache[2] != kv_heads or cache[3] != dim:
+        raise ValueError(f"rotary: key_cache must be [blocks, page, {kv_heads}, {dim}]")
+    if value_cache.shape != cache:
+        raise ValueError("rotary: value_cache must be like key_cache")
+    kc, vc = key_cache.stride(), value_cache.stride()
+    if (kc[3] != 1 or vc[3] != 1) and dim > 1:
+        raise ValueError("rotary: the caches need a unit head-dim stride")
+    if key_cache.dtype != kind or value_cache.dtype != kind \
+            or key_cache.get_device() != index or value_cache.get_device() != index:
+        raise TypeError(f"rotary: the caches must be {kind} on {k.device}")
+    if slots.dim() != 1 or slots.shape[0] != tokens or slots.dtype != torch.int64 \
+            or slots.get_device() != index:
         raise ValueError(f"rotary: slots must be int64 [tokens] on {k.device}")
+    heads = 0
     if q is not None:
-        _heads("q", q, like)
+        _heads("q", q, k)
+        heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        else:
-            _heads("q_out", q_out, q, q.shape[1])
+            q_out = torch.empty(q.shape, dtype=kind, device=q.device)
+        elif q_out is not q:
+            _heads("q_out", q_out, q, heads)
     else:
         q_out = None
-    _call(q, q_out, k, None, v, key_cache, value_cache, slots, positions, frequencies,
-          interleaved, False, float(factor))
+    _scalars(k, positions, frequencies)
+    _lib.ready(k)
+    if tokens:
+        with _lib.on_device(index):
+            status = _lib.load_library().qsa_rotary(
+                *_side(q), heads, *_side(q_out), *_side(k), kv_heads, None, 0, 0, *_side(v),
+                key_cache.data_ptr(), kc[0], kc[1], kc[2],
+                value_cache.data_ptr(), vc[0], vc[1], vc[2], cache[0], cache[1],
+                slots.data_ptr(), slots.stride(0), tokens, dim, positions.data_ptr(),
+                positions.stride(0), frequencies.data_ptr(), 2 * frequencies.shape[0], factor,
+                interleaved, False, _DTYPES[kind], _lib.raw_stream(index))
+        if status:
+            _lib.check(status, "rotary")
     return q_out
 
 

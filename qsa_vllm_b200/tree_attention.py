@@ -26,38 +26,46 @@ def tree_attention_workspace_bytes(rows: int, num_requests: int, num_q_heads: in
 def check_tree_arguments(what: str, q, caches, block_table, seq_lens, query_start_loc,
                          tree_mask, max_query_len) -> None:
     """Types, shapes, strides and devices of what the tree operators share."""
-    dev = q.device
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"{what}: q must be bfloat16 or float16, got {q.dtype}")
-    if q.dim() != 3 or (q.stride(2) != 1 and q.shape[2] > 1):
+    kind, dev = q.dtype, q.get_device()
+    if kind not in _DTYPES:
+        raise TypeError(f"{what}: q must be bfloat16 or float16, got {kind}")
+    shape = q.shape
+    if len(shape) != 3 or (q.stride(2) != 1 and shape[2] > 1):
         raise ValueError(f"{what}: q must be [rows, heads, dim] with a unit dim stride")
+    first = caches[0][1].shape
     for name, c in caches:
-        if c.dtype != q.dtype or c.device != dev:
-            raise TypeError(f"{what}: {name} must be {q.dtype} on {dev}")
-        if c.dim() != 4 or c.shape != caches[0][1].shape or c.shape[3] != q.shape[2]:
-            raise ValueError(f"{what}: {name} must be [blocks, page, kv_heads, {q.shape[2]}]")
-        if c.stride(3) != 1 and c.shape[3] > 1:
+        if c.dtype != kind or c.get_device() != dev:
+            raise TypeError(f"{what}: {name} must be {kind} on {q.device}")
+        if len(first) != 4 or c.shape != first or first[3] != shape[2]:
+            raise ValueError(f"{what}: {name} must be [blocks, page, kv_heads, {shape[2]}]")
+        if c.stride(3) != 1 and first[3] > 1:
             raise ValueError(f"{what}: {name} needs a unit head-dim stride")
     for name, t in (("block_table", block_table), ("seq_lens", seq_lens),
                     ("query_start_loc", query_start_loc)):
-        if t.dtype != torch.int32 or t.device != dev:
-            raise TypeError(f"{what}: {name} must be int32 on {dev}")
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
+        if t.dtype != torch.int32 or t.get_device() != dev:
+            raise TypeError(f"{what}: {name} must be int32 on {q.device}")
+        if t.dim() == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
             raise ValueError(f"{what}: {name} needs a unit stride over its last dim")
-    if block_table.dim() != 2 or seq_lens.shape != block_table.shape[:1] \
-            or query_start_loc.dim() != 1 \
-            or query_start_loc.shape[0] != block_table.shape[0] + 1:
+    table, lens, start = block_table.shape, seq_lens.shape, query_start_loc.shape
+    if len(table) != 2 or len(lens) != 1 or lens[0] != table[0] or len(start) != 1 \
+            or start[0] != table[0] + 1:
         raise ValueError(f"{what}: block_table [B, width], seq_lens [B] and query_start_loc "
                          "[B + 1] expected")
     if tree_mask is not None:
-        if tree_mask.dtype not in (torch.bool, torch.uint8) or tree_mask.device != dev:
-            raise TypeError(f"{what}: tree_mask must be bool or uint8 on {dev}")
-        if tree_mask.dim() != 2 or tree_mask.shape[0] != q.shape[0] \
-                or (tree_mask.stride(1) != 1 and tree_mask.shape[1] > 1):
+        if tree_mask.dtype not in (torch.bool, torch.uint8) or tree_mask.get_device() != dev:
+            raise TypeError(f"{what}: tree_mask must be bool or uint8 on {q.device}")
+        mask = tree_mask.shape
+        if len(mask) != 2 or mask[0] != shape[0] or (tree_mask.stride(1) != 1 and mask[1] > 1):
             raise ValueError(f"{what}: tree_mask must be [rows, drafted tokens] with a unit "
                              "stride over the tokens")
     if max_query_len < 1:
         raise ValueError(f"{what}: max_query_len must be positive")
+
+
+def check_lse(what: str, lse, q) -> None:
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] \
+            or lse.get_device() != q.get_device() or (lse.stride(1) != 1 and lse.shape[1] > 1):
+        raise ValueError(f"{what}: lse must be float32 [rows, heads] with a unit head stride")
 
 
 def mask_arguments(tree_mask: torch.Tensor | None, any_tensor: torch.Tensor) -> tuple:
@@ -90,37 +98,37 @@ def tree_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     max_query_len = int(max_query_len)
     check_tree_arguments(what, q, (("k_cache", k_cache), ("v_cache", v_cache)), block_table,
                          seq_lens, query_start_loc, tree_mask, max_query_len)
-    dev = q.device
-    rows, hq, d = q.shape
+    rows, hq, d = shape = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev \
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype != q.dtype or out.get_device() != q.get_device() \
             or (out.stride(2) != 1 and d > 1):
         raise ValueError(f"{what}: out must be like q, with a unit dim stride")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2]
-                            or lse.device != dev or (lse.stride(1) != 1 and hq > 1)):
-        raise ValueError(f"{what}: lse must be float32 [rows, heads] with a unit head stride")
-    _lib.ensure_device(dev)
+    if lse is not None:
+        check_lse(what, lse, q)
+    index = _lib.ready(q)
     if not rows:
         return out
     q = aligned_head_rows(q)
-    requests, hkv = block_table.shape[0], k_cache.shape[2]
-    need = tree_attention_workspace_bytes(rows, requests, hq, hkv, d, max_query_len)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        _lib.check(_lib.load_library().qsa_tree_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), rows, hq, d, _DTYPES[q.dtype],
-            k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-            v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
-            k_cache.shape[0], k_cache.shape[1], hkv,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], requests,
+    requests, width = block_table.shape
+    blocks, page, hkv, _ = k_cache.shape
+    qs, ks, vs, os = q.stride(), k_cache.stride(), v_cache.stride(), out.stride()
+    lib = _lib.load_library()
+    with _lib.on_device(index):
+        need = lib.qsa_tree_attention_workspace_bytes(rows, requests, hq, hkv, d, max_query_len)
+        if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        status = lib.qsa_tree_attention(
+            q.data_ptr(), qs[0], qs[1], rows, hq, d, _DTYPES[q.dtype],
+            k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+            blocks, page, hkv, block_table.data_ptr(), block_table.stride(0), width, requests,
             seq_lens.data_ptr(), query_start_loc.data_ptr(),
             *mask_arguments(tree_mask, seq_lens), max_query_len,
-            d ** -0.5 if scale is None else float(scale),
-            out.data_ptr(), out.stride(0), out.stride(1),
+            d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1],
             None if lse is None else lse.data_ptr(), 0 if lse is None else lse.stride(0),
-            workspace.data_ptr() if need else None, need, _lib.stream_ptr(dev)), what)
+            workspace.data_ptr() if need else None, need, _lib.raw_stream(index))
+    if status:
+        _lib.check(status, what)
     return out
 
 
