@@ -441,7 +441,7 @@ QSA_API size_t qsa_tree_attention_workspace_bytes(int32_t rows, int32_t num_requ
  * aligned rows of q and caches.  head_dim a multiple of 8 up to 256; head_dim
  * 64 / 128 with pages that are a multiple of 8 run on the tensor cores.
  * max_query_len sizes the work split (the longest request's rows; a smaller
- * value costs speed, not results).
+ * value costs speed, not results).  table_width * page_size at most 2^30.
  */
 QSA_API int qsa_tree_attention(
     const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t rows, int32_t num_q_heads,
@@ -490,7 +490,8 @@ QSA_API int qsa_attention_weights(
  * found through block_table [num_requests, table_width]; destinations through
  * out_table, or block_table again when out_table is NULL (in place).
  * In place each list must be strictly ascending over its entries that are not
- * below 0, and no source may lie below its destination.  With an out_table,
+ * below 0, no source may lie below its destination, and no page may be another
+ * request's too (move requests that share a prefix to pages of their own).  With an out_table,
  * destinations must not be pages that the call also reads.
  * Entries outside the tables or on unmapped pages, and in-place sources below
  * their destination, are skipped and set QSA_DEVICE_ERR_OUT_OF_RANGE.

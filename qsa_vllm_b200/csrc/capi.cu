@@ -939,6 +939,8 @@ static int tree_common(TreeParams& p, const char* who, const void* q, int64_t q_
                 num_kv_heads);
   if (page_size <= 0 || num_blocks < 0 || table_width < 0)
     return fail(QSA_ERR_INVALID, "%s: bad page geometry", who);
+  if (static_cast<int64_t>(table_width) * page_size > (int64_t{1} << 30))
+    return fail(QSA_ERR_UNSUPPORTED, "%s: tables of more than 2^30 tokens", who);
   if (!(scale > 0.0f) || !std::isfinite(scale))
     return fail(QSA_ERR_INVALID, "%s: scale must be positive and finite", who);
   if (num_requests == 0) return QSA_OK;
@@ -976,7 +978,7 @@ static int tree_common(TreeParams& p, const char* who, const void* q, int64_t q_
   p.mask_width = mask_width;
   p.scale = scale;
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-  p.max_query_len = max_query_len;
+  p.max_query_len = std::min(max_query_len, std::max(rows, 1));
   p.err = device_error_word();
   return QSA_OK;
 }

@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kGenThreads) attention_weights_general(TreePar
 
 size_t tree_attention_workspace(int rows, int requests, int q_heads, int kv_heads, int dim,
                                 int max_query_len) {
-  return tree_attention_tc_workspace(q_heads / kv_heads, dim, max_query_len);
+  return tree_attention_tc_workspace(q_heads / kv_heads, dim, std::min(max_query_len, rows));
 }
 
 cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t stream) {

@@ -64,8 +64,9 @@ struct PieceInfo {
   int64_t total;  // tiles of all units
   int64_t base;   // first tile of the unit
   int tiles;      // tiles of the unit
-  int b, h, grp;
-  int ranges;     // ranges in use
+  int row0, count;  // the request's packed rows
+  int h, grp;
+  int ranges;       // ranges in use
   int valid;
 };
 
@@ -116,6 +117,7 @@ struct TreeSmem {
   float2 ml[kTile];              // (m, l) of the second softmax warpgroup
   int64_t scan[kTreeThreads / 32];
   int64_t first_base;
+  TreeRequest first_r;           // of the range's first tile
   int first_b;
   int bad[2];                    // number of the piece that met infinite or NaN values
   uint32_t tmem_base;
@@ -146,14 +148,18 @@ __device__ __forceinline__ int64_t head_tiles(const TreeParams& p, const TreeReq
   return n;
 }
 
+__device__ __forceinline__ void unit_first(const TreeParams& p, TreeUnit& u, int span) {
+  u.h = u.grp = 0;
+  u.groups = (u.r.count + span - 1) / span;
+  u.tiles = unit_tiles(p, u.r, 0, span);
+}
+
 // Enters request b (or the next with rows); false past the last.
 __device__ __forceinline__ bool unit_enter(const TreeParams& p, TreeUnit& u, int span) {
   for (; u.b < p.requests; ++u.b) {
     u.r = tree_request_info(p, u.b);
     if (u.r.count == 0) continue;
-    u.h = u.grp = 0;
-    u.groups = (u.r.count + span - 1) / span;
-    u.tiles = unit_tiles(p, u.r, 0, span);
+    unit_first(p, u, span);
     return true;
   }
   return false;
@@ -173,11 +179,12 @@ __device__ __forceinline__ bool unit_next(const TreeParams& p, TreeUnit& u, int 
 }
 
 // The unit that holds tile `begin`, from the request that holds it.
-__device__ __forceinline__ bool unit_seek(const TreeParams& p, TreeUnit& u, int b, int64_t base,
-                                          int64_t begin, int span) {
+__device__ __forceinline__ bool unit_seek(const TreeParams& p, TreeUnit& u, const TreeRequest& r,
+                                          int b, int64_t base, int64_t begin, int span) {
+  u.r = r;
   u.b = b;
   u.base = base;
-  if (!unit_enter(p, u, span)) return false;
+  unit_first(p, u, span);
   const int64_t per_head = head_tiles(p, u.r, span);
   u.h = static_cast<int>((begin - base) / per_head);
   u.base += u.h * per_head;
@@ -369,9 +376,12 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
   // range's first tile names its request.
   const int per = (p.requests + kTreeThreads - 1) / kTreeThreads;
   int64_t mine = 0;
+  TreeRequest info_r{};  // of the run's last request: of all of it, for up to 320 requests
   for (int k = 0; k < per; ++k) {
     const int b = tid * per + k;
-    if (b < p.requests) mine += p.kv_heads * head_tiles(p, tree_request_info(p, b), span);
+    if (b >= p.requests) break;
+    info_r = tree_request_info(p, b);
+    mine += p.kv_heads * head_tiles(p, info_r, span);
   }
   int64_t incl = mine;
 #pragma unroll
@@ -401,11 +411,13 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     int64_t at = before;
     for (int k = 0; k < per; ++k) {
       const int b = tid * per + k;
+      if (per > 1 && b < p.requests) info_r = tree_request_info(p, b);
       const int64_t n =
-          b < p.requests ? p.kv_heads * head_tiles(p, tree_request_info(p, b), span) : 0;
+          per == 1 ? mine : b < p.requests ? p.kv_heads * head_tiles(p, info_r, span) : 0;
       if (begin < at + n) {
         sm.first_b = b;
         sm.first_base = at;
+        sm.first_r = info_r;
         break;
       }
       at += n;
@@ -441,9 +453,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     const int boxes = kTile / g.box_rows;
     const uint32_t box_bytes = g.box_rows * 128;
     TreeUnit u;
-    bool more = unit_seek(p, u, sm.first_b, sm.first_base, begin, span);
+    bool more = unit_seek(p, u, sm.first_r, sm.first_b, sm.first_base, begin, span);
     if (lane == 0) {
-      PieceInfo info = {total, u.base, u.tiles, u.b, u.h, u.grp, ranges, begin > u.base};
+      PieceInfo info = {total, u.base, u.tiles, u.r.row0, u.r.count, u.h, u.grp, ranges,
+                        begin > u.base};
       g.info[blockIdx.x] = info;
     }
     for (;; ++piece) {
@@ -451,6 +464,15 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
       const int t0 = static_cast<int>(max(begin - u.base, static_cast<int64_t>(0)));
       const int t1 = static_cast<int>(min(end - u.base, static_cast<int64_t>(u.tiles)));
       const int first = (u.grp * g.cohort + member) * C::kStreams * R;
+      const int32_t* table = p.table + (more ? u.b : 0) * p.table_stride;
+      auto page_of = [&](int tile, int& at) {
+        const int t = tile * kTile + lane * g.box_rows;
+        int q;
+        p.page_div.divmod(t, q, at);
+        return lane < boxes && t < u.r.tokens ? ld_once(table + q) : -1;
+      };
+      int at_next = 0, page_next = -1;
+      if (more) page_next = page_of(t0, at_next);
       ok = __all_sync(0xffffffffu, wait(&sm.q_empty, (piece & 1) ^ 1));
       if (!ok) break;
       if (lane == 0) {
@@ -469,17 +491,9 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             tma_load_4d(sm.q[s] + c * C::kSubBytes, &qmap, c * 64, 0, u.h,
                         u.r.row0 + first + s * R, &sm.q_full);
       }
-      const int32_t* table = p.table + u.b * p.table_stride;
-      auto page_of = [&](int tile, int& at) {
-        const int t = tile * kTile + lane * g.box_rows;
-        int q;
-        p.page_div.divmod(t, q, at);
-        int page = lane < boxes && t < u.r.tokens ? ld_once(table + q) : -1;
-        return page >= 0 && page < p.num_blocks ? page : -1;
-      };
-      int at_next, page_next = page_of(t0, at_next);
       for (int t = t0; t < t1; ++t, ++n) {
-        const int page = page_next, at = at_next;
+        const int page = page_next >= 0 && page_next < p.num_blocks ? page_next : -1;
+        const int at = at_next;
         if (t + 1 < t1) page_next = page_of(t + 1, at_next);
         const uint32_t mapped = __ballot_sync(0xffffffffu, page >= 0);
 #pragma unroll
@@ -865,10 +879,14 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
               }
             }
           } else {
-            uint4* out = reinterpret_cast<uint4*>(g.part_o + part_row * D + k);
+            // whole 32-byte sectors: rows are 4 D bytes apart from lane to lane
+            float* out = g.part_o + part_row * D + k;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              out[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 32; e += 8)
+              asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + e),
+                           "r"(o[e]), "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3]), "r"(o[e + 4]),
+                           "r"(o[e + 5]), "r"(o[e + 6]), "r"(o[e + 7])
+                           : "memory");
           }
         }
         if (live) {
@@ -914,9 +932,8 @@ tree_merge_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ 
   const int R = g.rows_per_tile;
   int local, head;
   g.group_div.divmod(row & (kTile - 1), local, head);
-  const TreeRequest r = tree_request_info(p, info.b);
   const int i = ((info.grp * g.cohort + member) * streams + row / kTile) * R + local;
-  if (local >= R || i >= r.count) return;
+  if (local >= R || i >= info.count) return;
   int last = first;  // one past the last range of the unit
   while (last < info.ranges && info.total * last / info.ranges < info.base + info.tiles) ++last;
   auto slot = [&](int k) {  // k-th piece, from the range before on
@@ -951,7 +968,7 @@ tree_merge_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ 
     }
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  const int64_t packed = r.row0 + i;
+  const int64_t packed = info.row0 + i;
   const int q_head = info.h * p.group + head;
   uint16_t* out = static_cast<uint16_t*>(p.out) + packed * p.out_row_stride +
                   q_head * p.out_head_stride + lane * kPer;

@@ -131,8 +131,8 @@ def cache_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: tor
 
     k_cache / v_cache: ``[blocks, page, H_kv, d]``; block_table, out_table: int32 ``[B, width]``;
     indices: int32 ``[B, n]`` or ``[B, H_kv, n]``, negative entries move nothing; starts: int32
-    ``[B]`` (0 where None).  Without ``out_table`` the move is in place: lists ascend, and no
-    token moves to a higher number.  With it, destinations are pages that the call does not
+    ``[B]`` (0 where None).  Without ``out_table`` the move is in place: lists ascend, no token
+    moves to a higher number, and no two requests share a page.  With it, destinations are pages that the call does not
     read.  Entries outside the tables or on unmapped pages are skipped and set the device error
     word."""
     what = "cache_compact"

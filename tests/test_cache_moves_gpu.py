@@ -175,6 +175,29 @@ def test_evict(dev, in_place, lengths, capacity, budget, sinks, recent, page, hk
     assert _lib.device_error_poll() == 0
 
 
+@pytest.mark.parametrize("cache_in_place", [True, False])
+def test_evict_with_one_of_cache_and_weights_in_place(dev, cache_in_place):
+    from qsa_vllm_b200.eviction import cache_evict
+    g = torch.Generator().manual_seed(5)
+    k, v, table, other = pool(g, dev, 3, 900, 16, 2, 128, BF16, 57)
+    w = torch.rand(3, 2, 900, generator=g).to(dev)
+    lengths, budget = [900, 640, 500], 600
+    keep = [[chosen(w[b, h].cpu(), n, budget, 4, 64) for h in range(2)]
+            for b, n in enumerate(lengths)]
+    want = moved(k, v, table, table if cache_in_place else other, keep, [0] * 3)
+    w_out = torch.zeros_like(w) if cache_in_place else w
+    w_want = torch.zeros(3, 2, 900) if cache_in_place else w.cpu().clone()
+    for b, n in enumerate(lengths):
+        for h in range(2):
+            w_want[b, h, :len(keep[b][h])] = w[b, h].cpu()[keep[b][h]]
+            w_want[b, h, len(keep[b][h]):n] = 0
+    seq = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    cache_evict(w, seq, table, k, v, budget, sinks=4, recent=64,
+                out_table=None if cache_in_place else other, weights_out=w_out)
+    assert torch.equal(w_out.cpu(), w_want)
+    assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+
+
 def test_evict_captured_again_and_again(dev):
     """A captured step that grows and evicts: the lengths are the device's, not the capture's."""
     from qsa_vllm_b200.eviction import cache_evict

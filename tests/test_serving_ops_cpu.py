@@ -166,3 +166,101 @@ def test_cache_move_c_abi_refusals():
             (dict(ws=None), 3, b"workspace"), (dict(n=100), 3, b"workspace"),
             (dict(ws=4100), 1, b"aligned"), (dict(cap=65, heads=1, stride=64), 1, b"stride")):
         assert evict(**bad) == status and word in lib.qsa_last_error(), bad
+
+
+def _tree(rows=5, hq=4, hkv=2, d=64, dtype=BF16):
+    k, v, table = _cache(hkv=hkv, d=d, dtype=dtype)
+    return dict(q=torch.zeros(rows, hq, d, dtype=dtype), k_cache=k, v_cache=v, block_table=table,
+                seq_lens=torch.zeros(2, dtype=torch.int32),
+                query_start_loc=torch.tensor([0, 2, 5], dtype=torch.int32), max_query_len=3)
+
+
+@pytest.mark.parametrize("error,change", [
+    (TypeError, dict(q=torch.zeros(5, 4, 64))),
+    (TypeError, dict(q=torch.zeros(5, 4, 64, dtype=torch.float16))),
+    (ValueError, dict(q=torch.zeros(5, 4, 32, dtype=BF16))),
+    (ValueError, dict(q=torch.zeros(5, 64, 4, dtype=BF16).transpose(1, 2))),
+    (ValueError, dict(q=torch.zeros(5, 64, dtype=BF16))),
+    (TypeError, dict(block_table=torch.zeros(2, 4, dtype=torch.int64))),
+    (ValueError, dict(block_table=torch.zeros(3, 4, dtype=torch.int32))),
+    (ValueError, dict(block_table=torch.zeros(4, 2, dtype=torch.int32).t())),
+    (TypeError, dict(seq_lens=torch.zeros(2))),
+    (ValueError, dict(seq_lens=torch.zeros((), dtype=torch.int32))),
+    (ValueError, dict(query_start_loc=torch.zeros(2, dtype=torch.int32))),
+    (TypeError, dict(tree_mask=torch.zeros(5, 3))),
+    (ValueError, dict(tree_mask=torch.zeros(4, 3, dtype=torch.bool))),
+    (ValueError, dict(tree_mask=torch.zeros(3, 5, dtype=torch.bool).t())),
+    (ValueError, dict(max_query_len=0)),
+    (ValueError, dict(out=torch.zeros(5, 4, 64))),
+    (ValueError, dict(lse=torch.zeros(5, 3))),
+    (ValueError, dict(lse=torch.zeros(5, 4, dtype=torch.float64))),
+    (ValueError, dict(v_cache=torch.zeros(7, 16, 2, 64, dtype=BF16))),
+])
+def test_tree_attention_refusals(error, change):
+    from qsa_vllm_b200.tree_attention import tree_paged_attention
+    with pytest.raises(error):
+        tree_paged_attention(**{**_tree(), **change})
+
+
+def test_tree_attention_needs_the_device():
+    from qsa_vllm_b200 import QSAError
+    from qsa_vllm_b200.tree_attention import tree_paged_attention
+    with pytest.raises(QSAError):
+        tree_paged_attention(**_tree(), tree_mask=torch.zeros(5, 3, dtype=torch.bool),
+                             lse=torch.zeros(5, 4))
+
+
+@pytest.mark.parametrize("error,change", [
+    (TypeError, dict(weights=torch.zeros(2, 2, 64, dtype=torch.float64))),
+    (ValueError, dict(weights=torch.zeros(2, 1, 64))),
+    (ValueError, dict(weights=torch.zeros(2, 64, 2).transpose(1, 2))),
+    (ValueError, dict(out=torch.zeros(2, 2, 63))),
+    (ValueError, dict(lse=torch.zeros(4, 4))),
+    (ValueError, dict(row_factors=torch.zeros(4))),
+    (ValueError, dict(row_factors=torch.zeros(5, dtype=torch.float64))),
+    (ValueError, dict(max_query_len=-1)),
+])
+def test_attention_weights_refusals(error, change):
+    from qsa_vllm_b200 import QSAError
+    from qsa_vllm_b200.eviction import accumulate_attention_weights
+    args = _tree()
+    del args["v_cache"]
+    args.update(lse=torch.zeros(5, 4), weights=torch.zeros(2, 2, 64))
+    with pytest.raises(QSAError):
+        accumulate_attention_weights(**args)
+    with pytest.raises(error):
+        accumulate_attention_weights(**{**args, **change})
+
+
+def test_tree_c_abi_refusals():
+    from qsa_vllm_b200 import _lib
+    lib = _lib.load_library()
+
+    def tree(rows=4, hq=8, d=128, dtype=0, k=4096, blocks=8, page=16, hkv=2, table=4096, width=4,
+             requests=2, mask=None, mask_width=0, most=2, scale=0.1, out=4096, v=4096, q=4096,
+             ws=None, n=0):
+        return lib.qsa_tree_attention(
+            q, hq * d, d, rows, hq, d, dtype, k, 64, 64, 64, v, 64, 64, 64, blocks, page, hkv, table,
+            4, width, requests, 4096, 4096, mask, 0, mask_width, most, scale, out, 8, 8, None, 0,
+            ws, n, None)
+    assert tree(rows=0) == 0 and tree(requests=0) == 0
+    for bad, status, word in (
+            (dict(rows=-1), 1, b"negative"), (dict(dtype=2), 2, b"dtype"), (dict(d=260), 2, b"head_dim"),
+            (dict(d=12), 2, b"head_dim"), (dict(d=0), 2, b"head_dim"), (dict(hq=7), 1, b"multiple"),
+            (dict(hkv=0), 1, b"multiple"), (dict(requests=40000), 2, b"65535"),
+            (dict(page=0), 1, b"page"), (dict(width=1 << 27), 2, b"2^30"),
+            (dict(scale=0.0), 1, b"scale"), (dict(scale=-1.0), 1, b"scale"),
+            (dict(scale=float("nan")), 1, b"scale"), (dict(scale=float("inf")), 1, b"scale"),
+            (dict(most=0), 1, b"max_query_len"), (dict(q=None), 1, b"null"),
+            (dict(table=None), 1, b"null"), (dict(out=None), 1, b"null"), (dict(v=None), 1, b"null"),
+            (dict(k=4104), 1, b"aligned"), (dict(q=4098), 1, b"aligned"), (dict(v=4104), 1, b"aligned"),
+            (dict(out=4097), 1, b"aligned"), (dict(), 3, b"workspace"),
+            (dict(ws=4096, n=100), 3, b"workspace")):
+        assert tree(**bad) == status and word in lib.qsa_last_error(), bad
+    assert lib.qsa_tree_attention_workspace_bytes(4, 2, 8, 2, 128, 2) > 0
+    # neither the longest request nor the batch makes it grow past two tiles of rows per block
+    most = lib.qsa_tree_attention_workspace_bytes(1 << 20, 2, 8, 2, 128, 1 << 30)
+    assert most <= 2 * 160 * 256 * 129 * 4 + 160 * 64
+    for bad in ((0, 2, 8, 2, 128, 2), (4, 0, 8, 2, 128, 2), (4, 2, 7, 2, 128, 2), (4, 2, 8, 2, 128, 0),
+                (4, 2, 8, 2, 72, 2)):
+        assert lib.qsa_tree_attention_workspace_bytes(*bad) == 0

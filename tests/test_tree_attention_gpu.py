@@ -218,6 +218,29 @@ def test_splits_of_long_contexts(dev):
                       poison=False))
 
 
+@pytest.mark.parametrize("requests,hq,hkv,d,page,most,mask", [
+    (700, 4, 2, 64, 16, 2, "chain"),     # more requests than the split scans at once
+    (150, 16, 8, 128, 16, 3, "random"),
+    (90, 8, 1, 128, 64, 40, "tree"),     # two row tiles
+    (60, 32, 1, 64, 8, 40, "random"),    # cohorts
+])
+def test_many_small_units(dev, requests, hq, hkv, d, page, most, mask):
+    """Many units to a block, most of a tile or two, some without rows, some without tokens."""
+    g = torch.Generator().manual_seed(requests)
+    lens = torch.randint(0, 300, (requests,), generator=g).tolist()
+    counts = torch.randint(0, most + 1, (requests,), generator=g).tolist()
+    c = tc.make(requests, lens, counts, hq, hkv, d, page, BF16, mask, dev, spread=1.2)
+    _, lse = check(c)
+    lse = torch.nan_to_num(lse, nan=0.0, neginf=-torch.inf)
+    w = torch.rand(requests, hkv, 290, generator=g).to(dev)
+    factors = (torch.rand(c["q"].shape[0], generator=g) < 0.5).float().to(dev)
+    want, tol = tc.weights(c, lse, w, factors)
+    got = accumulate(c, lse, w, torch.zeros_like(w), row_factors=factors)
+    for b, n in enumerate(lens):
+        n = min(n, 290)
+        tc.compare(got[b, :, :n], want[b, :, :n], tol[b, :, :n], f"request {b}")
+
+
 def test_offsets_past_32_bits(dev):
     """A cache of more than 2^32 bytes and 2^31 elements, its pages at both ends used."""
     page, hkv, d = 64, 8, 128
@@ -349,6 +372,23 @@ def test_weights_of_unmapped_pages_and_rows_left_out(dev, page, d):
     assert (w[0, :, page:2 * page] == 0).all()
     rows = torch.tensor([5, 3, 4]) * 4.0  # counted rows x heads of a group
     assert (w.sum(-1).cpu() - rows[:, None]).abs().max() < 1e-3
+
+
+@pytest.mark.parametrize("value", [-1.5, float("inf"), 1e-30, 3e38])
+@pytest.mark.parametrize("page", [16, 5])
+def test_weights_take_any_factor(dev, value, page):
+    c = tc.make(33, [300, 150], [9, 4], 8, 2, 64, page, BF16, "random", dev, poison=False)
+    _, lse = call(c)
+    lse = torch.nan_to_num(lse, neginf=-torch.inf)
+    factors = torch.ones(13, device=dev)
+    factors[[2, 11]] = value
+    got = accumulate(c, lse, torch.zeros(2, 2, 300, device=dev), row_factors=factors)
+    want, tol = tc.weights(c, lse, torch.zeros(2, 2, 300), factors)
+    fine = want.isfinite()
+    assert torch.equal(got.isfinite().cpu(), fine & (want.abs() < 3.4e38))
+    fine &= want.abs() < 3.4e38
+    tc.compare(torch.where(fine.to(dev), got, 0.0), torch.where(fine, want, 0.0),
+               torch.where(fine, tol, 0.0), "weights")
 
 
 def test_weights_without_rows_copy(dev):

@@ -149,7 +149,8 @@ def weights(c, lse, before, factors=None, scale=None):
         f = torch.ones(s.shape[0]).double() if factors is None else factors.double().cpu()[rows]
         use = ok & ~z.isinf()[..., None] & (f != 0)[:, None, None]
         e = torch.where(use, s - z.masked_fill(z.isinf(), 0)[..., None], -math.inf).exp()
-        e = e * torch.where(f != 0, f, 0.0)[:, None, None]
+        # an unseen token gets nothing, of an infinite factor either
+        e = torch.where(use, e * f[:, None, None], 0.0)
         n = min(s.shape[2], got.shape[2])
         delta = d * 2.0 ** -24 * a + 1.5 * 2.0 ** -23 * (
             s.abs() + z.masked_fill(z.isinf(), 0).abs()[..., None]) + 2.0 ** -21
