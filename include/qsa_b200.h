@@ -8,14 +8,21 @@
  *                            token (or physical slot) ids plus the causal tail
  *   3. qsa_sparse_attention  paged BF16 GQA attention over the selected tokens
  *
+ * and, for serving with the same paged caches: qsa_rotary (rotary positions,
+ * with the store to the cache), qsa_tree_attention (dense attention of decode
+ * rows, drafted-token trees and prompt chunks), qsa_attention_weights,
+ * qsa_cache_evict and qsa_cache_compact (keeping the cache small).
+ *
  * Conventions (every entry point):
  *   - All pointers are device pointers of the current CUDA device, except
  *     where a comment says otherwise.  bf16 tensors are passed as void*.
  *   - Strides are in ELEMENTS of the pointed-to type, as torch reports them.
  *   - `stream` is a cudaStream_t (NULL = legacy default stream).  Nothing
  *     synchronises the host; every launch is CUDA-graph capturable.
- *   - No entry point allocates device memory.  Attention takes a
- *     caller-provided workspace sized by qsa_sparse_attention_workspace_bytes.
+ *   - No entry point allocates device memory.  The attention entry points and
+ *     the eviction take a caller-provided workspace sized by the matching
+ *     *_workspace_bytes query; nothing in it has to start at zero or outlives
+ *     the call, and calls that do not overlap on the GPU may share one.
  *   - Return value: QSA_OK or a QSA_ERR_* code; qsa_last_error() gives the
  *     detail for the calling host thread.  Invalid metadata VALUES (a -1 page,
  *     an out-of-range index) are not errors: they are masked exactly as the

@@ -16,6 +16,15 @@
 // products N/2 cycles of the tensor core's 8192 flops, its exponentials
 // 8 N cycles of a scheduler's special-function unit.
 //
+// Measured on a B200: 64 requests of 8k-32k tokens, 16 rows of which 40%
+// count, 32 query heads over 4 KV heads of 128: 267 us, of which 226 remain
+// without the epilogue's arithmetic; the floor at a copy's rate is 212 us.
+// What mattered: columns without branches between them (373 -> 355 us), four
+// score buffers, mask bits per row and factors folded into the exponents
+// (-> 307), weights prefetched into L2 well ahead (-> 267): with 128 KB of
+// keys in flight per SM a load from memory waits behind them for longer than
+// two tiles take.
+//
 // Roles: warp 0 loads key tiles page by page with TMA into a ring; one lane of
 // warp 1 issues the products; warps 2-5 and 6-9 gather the pairs of a piece,
 // and take alternate tiles.  Work split: the (request, KV head) units, each of

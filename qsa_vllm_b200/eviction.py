@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .qsa import aligned_head_rows
-from .tree_attention import check_lse, check_tree_arguments, mask_arguments
+from .tree_attention import check_lse, check_tree_arguments
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -80,12 +80,10 @@ def accumulate_attention_weights(
     H_kv, capacity]``; out is weights itself (in place) where None.  Tokens from
     ``min(seq_lens[b], capacity)`` on are not written."""
     what = "accumulate_attention_weights"
-    max_query_len = int(max_query_len)
-    check_tree_arguments(what, q, (("k_cache", k_cache),), block_table, seq_lens,
-                         query_start_loc, tree_mask, max_query_len)
+    keys, _, tables = check_tree_arguments(what, q, k_cache, None, block_table, seq_lens,
+                                           query_start_loc, tree_mask, max_query_len)
     rows, hq, d = q.shape
-    requests, width = block_table.shape
-    blocks, page, hkv, _ = k_cache.shape
+    hkv, requests = tables[2], tables[6]
     dev = q.get_device()
     if out is None:
         out = weights
@@ -106,14 +104,10 @@ def accumulate_attention_weights(
     _lib.ready(q)
     if rows:
         q = aligned_head_rows(q)
-    qs, ks = q.stride(), k_cache.stride()
+    qs = q.stride()
     with _lib.on_device(dev):
         status = _lib.load_library().qsa_attention_weights(
-            q.data_ptr(), qs[0], qs[1], rows, hq, d, _DTYPES[q.dtype],
-            k_cache.data_ptr(), ks[0], ks[1], ks[2], blocks, page, hkv,
-            block_table.data_ptr(), block_table.stride(0), width, requests,
-            seq_lens.data_ptr(), query_start_loc.data_ptr(),
-            *mask_arguments(tree_mask, seq_lens), max_query_len,
+            q.data_ptr(), qs[0], qs[1], rows, hq, d, _DTYPES[q.dtype], *keys, *tables,
             d ** -0.5 if scale is None else scale, lse.data_ptr(), lse.stride(0),
             None if row_factors is None else row_factors.data_ptr(),
             0 if row_factors is None else row_factors.stride(0),

@@ -66,46 +66,49 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str =
     return (f if device is None else f.to(device)), factor
 
 
-def _heads(name: str, t: torch.Tensor, like: torch.Tensor, heads: int | None = None) -> None:
-    """Refuses a tensor that is not [tokens, heads, dim] beside ``like``."""
-    shape, other = t.shape, like.shape
-    if len(shape) != 3 or shape[0] != other[0] or shape[2] != other[2] \
-            or (heads is not None and shape[1] != heads):
+def _heads(name: str, t: torch.Tensor, like: tuple, heads: int = 0) -> tuple:
+    """(pointer, row stride, head stride) of a tensor [tokens, heads, dim] that fits ``like``
+    (tokens, dim, dtype, device index)."""
+    shape, (row, head, unit) = t.shape, t.stride() if t.dim() == 3 else (0, 0, 0)
+    if len(shape) != 3 or shape[0] != like[0] or shape[2] != like[1] \
+            or (heads and shape[1] != heads):
         raise ValueError(f"rotary: {name} must be [tokens, heads, dim] matching the others, "
                          f"got {tuple(shape)}")
-    if t.dtype != like.dtype or t.get_device() != like.get_device():
-        raise TypeError(f"rotary: {name} must be {like.dtype} on {like.device}, "
-                        f"got {t.dtype} on {t.device}")
-    if t.stride(2) != 1 and shape[2] > 1:
+    if t.dtype != like[2] or t.get_device() != like[3]:
+        raise TypeError(f"rotary: {name} must be {like[2]} on the others' device, got {t.dtype} "
+                        f"on {t.device}")
+    if unit != 1 and like[1] > 1:
         raise ValueError(f"rotary: {name} needs a unit head-dim stride")
+    return t.data_ptr(), row, head
 
 
-def _scalars(like: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor) -> None:
-    """Refuses positions and frequencies that do not fit ``like``."""
-    if like.dtype not in _DTYPES:
-        raise TypeError(f"rotary: bfloat16, float16 or float32 expected, got {like.dtype}")
-    if positions.dim() != 1 or positions.shape[0] != like.shape[0] \
-            or positions.dtype != torch.int64:
+def _like(t: torch.Tensor) -> tuple:
+    if t.dim() != 3:
+        raise ValueError("rotary: queries and keys must be [tokens, heads, dim]")
+    shape = t.shape
+    return shape[0], shape[2], t.dtype, t.get_device()
+
+
+def _scalars(like: tuple, positions: torch.Tensor, frequencies: torch.Tensor) -> tuple:
+    """Pointers, stride and rotary dim of positions and frequencies that fit ``like``, and the
+    code of its dtype."""
+    kind = _DTYPES.get(like[2])
+    if kind is None:
+        raise TypeError(f"rotary: bfloat16, float16 or float32 expected, got {like[2]}")
+    if positions.dim() != 1 or positions.shape[0] != like[0] or positions.dtype != torch.int64:
         raise ValueError("rotary: positions must be int64 [tokens]")
     if frequencies.dim() != 1 or frequencies.dtype != torch.float64 \
             or not frequencies.is_contiguous():
         raise TypeError("rotary: frequencies must be a contiguous float64 vector")
-    if not 2 <= 2 * frequencies.shape[0] <= like.shape[2]:
-        raise ValueError(f"rotary: {frequencies.shape[0]} frequencies for a head of "
-                         f"{like.shape[2]}")
-    if positions.get_device() != like.get_device() \
-            or frequencies.get_device() != like.get_device():
-        raise TypeError(f"rotary: positions and frequencies must be on {like.device}")
+    rotary_dim = 2 * frequencies.shape[0]
+    if not 2 <= rotary_dim <= like[1]:
+        raise ValueError(f"rotary: {rotary_dim // 2} frequencies for a head of {like[1]}")
+    if positions.get_device() != like[3] or frequencies.get_device() != like[3]:
+        raise TypeError("rotary: positions and frequencies must be on the others' device")
+    return positions.data_ptr(), positions.stride(0), frequencies.data_ptr(), rotary_dim, kind
 
 
-def _side(x: torch.Tensor | None) -> tuple:
-    """Pointer, row and head stride."""
-    if x is None:
-        return None, 0, 0
-    strides = x.stride()
-    return x.data_ptr(), strides[0], strides[1]
-
-
+_NO_SIDE = (None, 0, 0)
 _NO_CACHE = (None, 0, 0, None, 0, 0, 0, None, 0, 0, 0, 0, 0, None, 0)
 
 
@@ -120,37 +123,37 @@ def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torc
     ``[tokens]``; frequencies: float64 ``[rotary_dim / 2]``.  ``q_out`` / ``k_out`` may be the
     inputs themselves (in place); other overlaps are not allowed.  New contiguous tensors are
     returned where they are None."""
-    like = q if q is not None else k
-    if like is None:
+    first = q if q is not None else k
+    if first is None:
         raise ValueError("rotary: q or k expected")
-    heads = [0, 0]
-    for i, (x, out) in enumerate(((q, q_out), (k, k_out))):
-        if x is None:
-            continue
-        _heads("k" if i else "q", x, like)
-        heads[i] = x.shape[1]
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            if i:
-                k_out = out
-            else:
-                q_out = out
-        elif out is not x:
-            _heads("k_out" if i else "q_out", out, x, heads[i])
-    if q is None:
+    like = _like(first)
+    tokens, dim, kind, index = like
+    q_side = q_to = k_side = k_to = _NO_SIDE
+    q_heads = k_heads = 0
+    if q is not None:
+        q_side = _heads("q", q, like)
+        q_heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=kind, device=q.device)
+        q_to = q_side if q_out is q else _heads("q_out", q_out, like, q_heads)
+    else:
         q_out = None
-    if k is None:
+    if k is not None:
+        k_side = _heads("k", k, like)
+        k_heads = k.shape[1]
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=kind, device=k.device)
+        k_to = k_side if k_out is k else _heads("k_out", k_out, like, k_heads)
+    else:
         k_out = None
-    _scalars(like, positions, frequencies)
-    index = _lib.ready(like)
-    tokens, _, dim = like.shape
+    pos, pos_step, freq, rotary_dim, code = _scalars(like, positions, frequencies)
+    _lib.ready(first)
     if tokens:
         with _lib.on_device(index):
             status = _lib.load_library().qsa_rotary(
-                *_side(q), heads[0], *_side(q_out), *_side(k), heads[1], *_side(k_out),
-                *_NO_CACHE, tokens, dim, positions.data_ptr(), positions.stride(0),
-                frequencies.data_ptr(), 2 * frequencies.shape[0], factor, interleaved, inverse,
-                _DTYPES[like.dtype], _lib.raw_stream(index))
+                *q_side, q_heads, *q_to, *k_side, k_heads, *k_to, *_NO_CACHE, tokens, dim, pos,
+                pos_step, freq, rotary_dim, factor, interleaved, inverse, code,
+                _lib.raw_stream(index))
         if status:
             _lib.check(status, "rotary")
     return q_out, k_out
@@ -168,10 +171,12 @@ def rotary_store(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     int64 ``[tokens]``, page * page_size + offset.  Tokens with a slot below 0 are not stored;
     one past the cache is not stored either and sets the device error word.  No two tokens may
     share a slot."""
-    _heads("k", k, k)
-    tokens, kv_heads, dim = k.shape
-    _heads("v", v, k, kv_heads)
-    cache, kind, index = key_cache.shape, k.dtype, k.get_device()
+    like = _like(k)
+    tokens, dim, kind, index = like
+    k_side = _heads("k", k, like)
+    kv_heads = k.shape[1]
+    v_side = _heads("v", v, like, kv_heads)
+    cache = key_cache.shape
     if len(cache) != 4 or cache[2] != kv_heads or cache[3] != dim:
         raise ValueError(f"rotary: key_cache must be [blocks, page, {kv_heads}, {dim}]")
     if value_cache.shape != cache:
@@ -185,27 +190,26 @@ def rotary_store(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     if slots.dim() != 1 or slots.shape[0] != tokens or slots.dtype != torch.int64 \
             or slots.get_device() != index:
         raise ValueError(f"rotary: slots must be int64 [tokens] on {k.device}")
+    q_side = q_to = _NO_SIDE
     heads = 0
     if q is not None:
-        _heads("q", q, k)
+        q_side = _heads("q", q, like)
         heads = q.shape[1]
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=kind, device=q.device)
-        elif q_out is not q:
-            _heads("q_out", q_out, q, heads)
+        q_to = q_side if q_out is q else _heads("q_out", q_out, like, heads)
     else:
         q_out = None
-    _scalars(k, positions, frequencies)
+    pos, pos_step, freq, rotary_dim, code = _scalars(like, positions, frequencies)
     _lib.ready(k)
     if tokens:
         with _lib.on_device(index):
             status = _lib.load_library().qsa_rotary(
-                *_side(q), heads, *_side(q_out), *_side(k), kv_heads, None, 0, 0, *_side(v),
+                *q_side, heads, *q_to, *k_side, kv_heads, None, 0, 0, *v_side,
                 key_cache.data_ptr(), kc[0], kc[1], kc[2],
                 value_cache.data_ptr(), vc[0], vc[1], vc[2], cache[0], cache[1],
-                slots.data_ptr(), slots.stride(0), tokens, dim, positions.data_ptr(),
-                positions.stride(0), frequencies.data_ptr(), 2 * frequencies.shape[0], factor,
-                interleaved, False, _DTYPES[kind], _lib.raw_stream(index))
+                slots.data_ptr(), slots.stride(0), tokens, dim, pos, pos_step, freq, rotary_dim,
+                factor, interleaved, False, code, _lib.raw_stream(index))
         if status:
             _lib.check(status, "rotary")
     return q_out
