@@ -11,7 +11,10 @@
 // Two softmax warpgroups work on S tiles of their own while the tensor core
 // runs the other's products.  DUAL (more rows than one tile holds): each has
 // rows of its own and both read the same key and value tiles.  Otherwise both
-// have the same rows and take alternate token tiles, joined at the end.
+// have the same rows and take alternate token tiles, joined at the end; with
+// heads of 64, up to 64 rows lie in the lower half of the first warpgroup's S and the upper
+// half of the second's, so that the two compute on different schedulers (61
+// single rows of heads of 64: 107 -> 99 us).
 //
 // Roles: warp 0 loads query, key and value tiles page by page with TMA into a
 // ring; one lane of warp 1 issues all tensor-core work; warps 2-5 and 6-9
@@ -35,8 +38,8 @@
 // memory the others find in L2.
 //
 // Measured on a B200.  64 requests of 8k-32k tokens, trees of 16, 32 query
-// heads over 4 KV heads of 128 (memory-bound): 472 us, 5.7 TB/s of keys and
-// values, 87% of a copy's rate; without the softmax arithmetic 441 us.  8
+// heads over 4 KV heads of 128 (memory-bound): 475 us, 5.7 TB/s of keys and
+// values, 87% of a copy's rate; without the softmax arithmetic 427 us.  8
 // requests of 131072 tokens, trees of 64 (twice 128 rows a KV head and CTA
 // pair): 980 us, 1.1 PFLOP/s at the 1.5 GHz that the power limit leaves; its
 // products alone take 785 us.  There a CTA's two row tiles spend 3400 cycles
@@ -98,8 +101,22 @@ struct TreeCfg {
   static constexpr int kSubBytes = kTile * 128;       // 16 KB
   static constexpr int kTileBytes = kSub * kSubBytes;
   static constexpr int kStreams = DUAL ? 2 : 1;       // row tiles
-  static constexpr int kFit = (224 * 1024 - kStreams * kTileBytes) / kTileBytes;
+  // Up to 64 rows of a single row tile, shifted apart: room for the second
+  // warpgroup's O.  Not for head dim 128, where it would cost a sixth of the
+  // ring (475 -> 550 us for the first shape above).
+  static constexpr bool kApart = !DUAL && D == 64;
+  static constexpr int kXchgBytes = kApart ? 64 * D * 4 : 16;
+  static constexpr int kFit =
+      (224 * 1024 - kStreams * kTileBytes - (kApart ? kXchgBytes : 0)) / kTileBytes;
   static constexpr int S = kFit > 10 ? 10 : kFit;
+  // Values follow their keys by kLag tiles through the ring.  With alternate
+  // tiles the product with the values of tile j comes between the scores of
+  // tiles j + 1 and j + 2; loaded beside their keys they would hold their
+  // places, and those of the keys behind them, for two tiles (487 us instead
+  // of 475 for the first shape above; two tiles later they are no better).
+  static constexpr int kLag = DUAL ? 0 : 1;
+  static __device__ __forceinline__ int key_pos(int n) { return n < kLag ? n : 2 * n - kLag; }
+  static __device__ __forceinline__ int value_pos(int n) { return 2 * n + kLag + 1; }
   static constexpr int kRows = kStreams * kTile;
 };
 
@@ -111,6 +128,7 @@ struct TreePiece {
   int region;  // tokens from here on are not seen by all of its rows
   int t0, t1;  // token tiles
   int tiles;   // of the whole unit
+  int shift;   // the second warpgroup's first row of S (single row tile)
   int end;     // no more pieces
 };
 // A piece's slot is written again four pieces later, when the products of the
@@ -127,6 +145,7 @@ struct TreeSmem {
   TreePiece piece[kPieceRing];
   alignas(16) uint32_t meta[kMetaRing][4];  // tokens of the tile that exist on mapped pages
   float2 ml[kTile];              // (m, l) of the second softmax warpgroup
+  float xo[C::kXchgBytes / 4];   // [column][row]: its O, when its rows are shifted
   int64_t scan[kTreeThreads / 32];
   int64_t first_base;
   TreeRequest first_r;           // of the range's first tile
@@ -231,8 +250,8 @@ struct RingPos {
   int slot;
   uint32_t phase;
   template <int S>
-  __device__ __forceinline__ void step() {
-    slot += 2;
+  __device__ __forceinline__ void step(int n) {
+    slot += n;
     if (slot >= S) {
       slot -= S;
       phase ^= 1;
@@ -471,6 +490,24 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
                         begin > u.base};
       g.info[blockIdx.x] = info;
     }
+    struct Place {  // this lane's box of a tile
+      int page, at, h;
+    };
+    Place past[C::kLag > 0 ? C::kLag : 1] = {};  // of the tiles whose values are to come
+    auto load = [&](const CUtensorMap* map, int pos, const Place& x) {
+      const int slot = pos % C::S;
+      ok = __all_sync(0xffffffffu, wait(&sm.empty[slot], ((pos / C::S) & 1) ^ 1));
+      if (!ok) return;
+      if (lane == 0) mbar_arrive_expect(&sm.full[slot], C::kTileBytes);
+      __syncwarp();
+      if (lane < boxes) {
+        uint8_t* dst = sm.ring[slot] + lane * box_bytes;
+#pragma unroll
+        for (int c = 0; c < C::kSub; ++c)
+          tma_load_4d(dst + c * C::kSubBytes, map, c * 64, x.h, x.at,
+                      x.page >= 0 ? x.page : p.num_blocks, &sm.full[slot]);
+      }
+    };
     for (;; ++piece) {
       more = more && u.base < end;
       const int t0 = static_cast<int>(max(begin - u.base, static_cast<int64_t>(0)));
@@ -483,64 +520,78 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         p.page_div.divmod(t, q, at);
         return lane < boxes && t < u.r.tokens ? ld_once(table + q) : -1;
       };
-      int at_next = 0, page_next = -1;
-      if (more) page_next = page_of(t0, at_next);
-      ok = __all_sync(0xffffffffu, wait(&sm.q_empty, (piece & 1) ^ 1));
-      if (!ok) break;
-      if (lane == 0) {
-        const int region =
-            max(p.mask != nullptr ? u.r.prefix : u.r.prefix + first + 1, 0);
-        sm.piece[piece % kPieceRing] =
-            TreePiece{u.r, u.b, u.h, first, region, t0, t1, u.tiles, !more};
-        mbar_arrive(&sm.piece_full[piece % kPieceRing]);
-      }
-      if (!more) break;
-      if (lane == 0) {
-        const int rows = R * p.group;
-        mbar_arrive_expect(&sm.q_full, C::kStreams * C::kSub * rows * 128);
-        for (int s = 0; s < C::kStreams; ++s)
-          for (int c = 0; c < C::kSub; ++c)
-            tma_load_4d(sm.q[s] + c * C::kSubBytes, &qmap, c * 64, 0, u.h,
-                        u.r.row0 + first + s * R, &sm.q_full);
-      }
-      for (int t = t0; t < t1; ++t, ++n) {
-        const int page = page_next >= 0 && page_next < p.num_blocks ? page_next : -1;
-        const int at = at_next;
-        if (t + 1 < t1) page_next = page_of(t + 1, at_next);
-        const uint32_t mapped = __ballot_sync(0xffffffffu, page >= 0);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int seq = 2 * n + kv, slot = seq % C::S;
-          ok = __all_sync(0xffffffffu, wait(&sm.empty[slot], ((seq / C::S) & 1) ^ 1));
-          if (!ok) break;
-          if (kv == 0 && lane < 4) {
-            uint32_t word;
-            if (g.box_rows >= 32) {
-              word = (mapped >> (lane * 32 / g.box_rows)) & 1 ? 0xffffffffu : 0u;
-            } else {
-              const int in_word = 32 / g.box_rows;
-              word = 0;
-              for (int k = 0; k < in_word; ++k)
-                if ((mapped >> (lane * in_word + k)) & 1)
-                  word |= ((1u << g.box_rows) - 1) << (k * g.box_rows);
-            }
-            const int left = u.r.tokens - t * kTile - lane * 32;
-            if (left < 32) word &= left <= 0 ? 0u : (1u << left) - 1;
-            sm.meta[n % kMetaRing][lane] = word;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect(&sm.full[slot], C::kTileBytes);
-          __syncwarp();
-          if (lane < boxes) {
-            uint8_t* dst = sm.ring[slot] + lane * box_bytes;
-#pragma unroll
-            for (int c = 0; c < C::kSub; ++c)
-              tma_load_4d(dst + c * C::kSubBytes, kv ? &vmap : &kmap, c * 64, u.h, at,
-                          page >= 0 ? page : p.num_blocks, &sm.full[slot]);
+      // the queries, once those of the piece before have been used: behind the
+      // first keys, as the last values of that piece come with them
+      bool handed = false;
+      auto hand_over = [&]() {
+        handed = true;
+        ok = __all_sync(0xffffffffu, wait(&sm.q_empty, (piece & 1) ^ 1));
+        if (!ok) return;
+        if (lane == 0) {
+          const int region =
+              max(p.mask != nullptr ? u.r.prefix : u.r.prefix + first + 1, 0);
+          sm.piece[piece % kPieceRing] =
+              TreePiece{u.r, u.b, u.h, first, region, t0, t1, u.tiles,
+                        C::kApart && min(u.r.count - first, R) * p.group <= 64 ? 64 : 0, !more};
+          mbar_arrive(&sm.piece_full[piece % kPieceRing]);
+          if (more) {
+            const int rows = R * p.group;
+            mbar_arrive_expect(&sm.q_full, C::kStreams * C::kSub * rows * 128);
+            for (int s = 0; s < C::kStreams; ++s)
+              for (int c = 0; c < C::kSub; ++c)
+                tma_load_4d(sm.q[s] + c * C::kSubBytes, &qmap, c * 64, 0, u.h,
+                            u.r.row0 + first + s * R, &sm.q_full);
           }
         }
-        if (!ok) break;
+        __syncwarp();
+      };
+      if (!more) {  // the last values, then the end
+        for (int k = C::kLag; k > 0 && ok; --k) {
+          if (n >= k) load(&vmap, C::value_pos(n - k), past[0]);
+          for (int x = 0; x + 1 < C::kLag; ++x) past[x] = past[x + 1];
+        }
+        if (ok) hand_over();
+        break;
       }
+      int at_next, page_next = page_of(t0, at_next);
+      for (int t = t0; t < t1; ++t, ++n) {
+        if (t - t0 == (piece > 0 ? C::kLag : 0)) hand_over();
+        if (!ok) break;
+        const Place place = {page_next >= 0 && page_next < p.num_blocks ? page_next : -1, at_next,
+                             u.h};
+        if (t + 1 < t1) page_next = page_of(t + 1, at_next);
+        const uint32_t mapped = __ballot_sync(0xffffffffu, place.page >= 0);
+        const int slot = C::key_pos(n) % C::S;
+        ok = __all_sync(0xffffffffu,
+                        wait(&sm.empty[slot], ((C::key_pos(n) / C::S) & 1) ^ 1));
+        if (!ok) break;
+        if (lane < 4) {
+          uint32_t word;
+          if (g.box_rows >= 32) {
+            word = (mapped >> (lane * 32 / g.box_rows)) & 1 ? 0xffffffffu : 0u;
+          } else {
+            const int in_word = 32 / g.box_rows;
+            word = 0;
+            for (int k = 0; k < in_word; ++k)
+              if ((mapped >> (lane * in_word + k)) & 1)
+                word |= ((1u << g.box_rows) - 1) << (k * g.box_rows);
+          }
+          const int left = u.r.tokens - t * kTile - lane * 32;
+          if (left < 32) word &= left <= 0 ? 0u : (1u << left) - 1;
+          sm.meta[n % kMetaRing][lane] = word;
+        }
+        __syncwarp();
+        load(&kmap, C::key_pos(n), place);
+        if constexpr (C::kLag == 0) {
+          if (ok) load(&vmap, C::value_pos(n), place);
+        } else {
+          if (ok && n >= C::kLag) load(&vmap, C::value_pos(n - C::kLag), past[0]);
+#pragma unroll
+          for (int x = 0; x + 1 < C::kLag; ++x) past[x] = past[x + 1];
+          past[C::kLag - 1] = place;
+        }
+      }
+      if (ok && !handed) hand_over();
       if (!ok) break;
       more = unit_next(p, u, span);
     }
@@ -548,8 +599,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     // copies in flight end before the block may
     if (!ok) mbar_wait(&sm.q_full, piece & 1);
     for (int k = 0; !ok && k < C::S; ++k) {
-      const int seq = 2 * n + 1 - k;
-      if (seq >= 0) mbar_wait(&sm.full[seq % C::S], (seq / C::S) & 1);
+      const int pos = C::key_pos(n) + 1 - k;
+      if (pos >= 0) mbar_wait(&sm.full[pos % C::S], (pos / C::S) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -562,12 +613,16 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
     const uint64_t q_desc = sw128_desc(smem_u32(sm.q[0]));
     const uint64_t k_desc = sw128_desc(smem_u32(sm.ring[0]));
     const uint64_t v_desc = value_desc(smem_u32(sm.ring[0]));
-    int piece = 0;
+    int piece = 0, shift = 0;
     uint32_t given[2] = {0, 0};  // P tiles taken of each softmax warpgroup
-    RingPos kp{0, 0}, vp{1, 0};
+    RingPos kp{0, 0}, vp{C::kLag + 1, 0};
+    int keys = 0;  // key tiles met
     auto qk = [&](int s) {
       if (leader) {
-        const uint64_t a = q_desc + (DUAL ? s : 0) * (C::kTileBytes >> 4);
+        // shifted rows: the tile begins 64 rows before the queries, with
+        // whatever lies there (the rows of S do not meet)
+        const uint64_t a = DUAL ? q_desc + s * (C::kTileBytes >> 4)
+                                : q_desc - (s ? static_cast<uint32_t>(shift) * 128 >> 4 : 0);
         const uint64_t b = k_desc + static_cast<uint32_t>(kp.slot) * (C::kTileBytes >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -599,6 +654,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
       ok = arrived(&sm.piece_full[piece % kPieceRing], piece / kPieceRing & 1);
       if (!ok || pc.end) break;
       const int m = pc.t1 - pc.t0;
+      shift = pc.shift;
       ok = arrived(&sm.q_full, piece & 1);
       if (!ok) break;
       if constexpr (DUAL) {
@@ -623,11 +679,11 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
           if (!ok) break;
           if (j > 0) {
             commit(&sm.empty[vp.slot]);
-            vp.template step<C::S>();
+            vp.template step<C::S>(2);
           }
           if (j < m) {
             commit(&sm.empty[kp.slot]);
-            kp.template step<C::S>();
+            kp.template step<C::S>(2);
           }
           if (j == m - 1) commit(&sm.q_empty);
         }
@@ -640,7 +696,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             tc_fence_after();
             pv(s, j >= 4);
             commit(&sm.empty[vp.slot]);
-            vp.template step<C::S>();
+            vp.template step<C::S>(2);
           }
           if (j < m) {
             if (j < 2) ok = k_in();
@@ -648,7 +704,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             tc_fence_after();
             qk(s);
             commit(&sm.empty[kp.slot]);
-            kp.template step<C::S>();
+            kp.template step<C::S>(keys++ < C::kLag ? 1 : 2);
             if (j == m - 1) commit(&sm.q_empty);
           }
         }
@@ -682,6 +738,10 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
       if (!ok || pc.end) break;
       const int t0 = pc.t0, t1 = pc.t1;
       const int region = pc.region;
+      // this thread's row of the row tile, and whether its warp has any
+      const int vrow = row - (st ? pc.shift : 0);
+      const int rows = min(pc.r.count - pc.first - (DUAL ? st * R : 0), R) * p.group;
+      const bool busy = vrow - lane < rows && vrow - lane >= 0;
       float m = -INFINITY, l = 0.0f;
       const int step = DUAL ? 1 : 2;
       bool fresh = true;
@@ -694,9 +754,9 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         const uint4 words = *reinterpret_cast<const uint4*>(sm.meta[seq % kMetaRing]);
         const bool masked = (t + 1) * kTile > region ||
                             (words.x & words.y & words.z & words.w) != 0xffffffffu;
-        if (masked) {
+        if (masked && busy) {
           uint32_t w[4] = {words.x, words.y, words.z, words.w};
-          row_mask(w, p, pc.r, t, pc.first + (DUAL ? st * R : 0), g.group_div.div(row), R, lane);
+          row_mask(w, p, pc.r, t, pc.first + (DUAL ? st * R : 0), g.group_div.div(vrow), R, lane);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // hidden scores become -inf in place
             uint32_t s[32];
@@ -708,9 +768,11 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             tmem_st32(ts + k * 32, s);
           }
           tmem_wait_st();
+        }
+        if (masked) {
           // Values of tokens that may not be read become 0; infinite or NaN
           // elements of drafted tokens too, and the piece remembers them.
-          const int vseq = 2 * seq + 1;
+          const int vseq = C::value_pos(seq);
           ok = __all_sync(0xffffffffu, wait(&sm.full[vseq % C::S], (vseq / C::S) & 1));
           if (!ok) break;
           constexpr int kParts = DUAL ? 2 : 1;   // threads of one token
@@ -755,6 +817,11 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         // far above (always in a piece's first tile, rarely later) it becomes
         // the one to take them against, and the pass is made again: S is
         // still whole, as P is only written behind this loop.
+        if (!busy) {  // P of rows that are none may be anything
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_ready[st]);
+          continue;
+        }
         uint32_t pk[kTile / 2];
         float2 sum;
         for (bool settled = false;;) {
@@ -795,9 +862,22 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
       ok = __all_sync(0xffffffffu, wait(&sm.o_full[st], piece & 1));
       if (!ok) break;
       float f0 = 1.0f, f1 = 0.0f;  // factors of this and the other warpgroup's O
+      const bool apart = C::kApart && pc.shift;  // the warpgroups' rows lie in other lanes
       if constexpr (!DUAL) {
         if (st == 1) {
-          sm.ml[row] = make_float2(m, l);
+          if (vrow >= 0) sm.ml[vrow] = make_float2(m, l);
+          if (apart && busy && tiles > 1) {
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < D; k += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + k, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) sm.xo[(k + e) * 64 + vrow] = __uint_as_float(o[e]);
+            }
+            tc_fence_before();
+          }
           mbar_arrive(&sm.xchg[0]);
           ok = __all_sync(0xffffffffu, wait(&sm.xchg[1], piece & 1));
           if (!ok) break;
@@ -818,9 +898,9 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         tc_fence_after();
         const TreeRequest r = pc.r;
         int local, head;
-        g.group_div.divmod(row, local, head);
+        g.group_div.divmod(max(vrow, 0), local, head);
         const int i = pc.first + (DUAL ? st * R : 0) + local;  // this thread's row of the request
-        const bool live = local < R && i < r.count;
+        const bool live = busy && local < R && i < r.count;
         const bool whole = tiles == pc.tiles;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const float lse2 = l == 0.0f ? -INFINITY : m * c + log2f(l);
@@ -837,7 +917,13 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
           if constexpr (!DUAL) {
             if (tiles > 1) {
               uint32_t o1[32];
-              tmem_ld32(tmem_o[1] + lane_off + k, o1);
+              if (apart) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  o1[e] = __float_as_uint(sm.xo[(k + e) * 64 + (row & 63)]);
+              } else {
+                tmem_ld32(tmem_o[1] + lane_off + k, o1);
+              }
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e)
