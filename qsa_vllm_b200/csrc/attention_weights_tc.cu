@@ -17,8 +17,9 @@
 // 8 N cycles of a scheduler's special-function unit.
 //
 // Measured on a B200: 64 requests of 8k-32k tokens, 16 rows of which 40%
-// count, 32 query heads over 4 KV heads of 128: 267 us, of which 226 remain
-// without the epilogue's arithmetic; the floor at a copy's rate is 212 us.
+// count, 32 query heads over 4 KV heads of 128: 284 us in long runs, 267 in
+// short ones, of which 226 remain without the epilogue's arithmetic; the floor
+// at a copy's rate is 213 us.
 // What mattered: columns without branches between them (373 -> 355 us), four
 // score buffers, mask bits per row and factors folded into the exponents
 // (-> 307), weights prefetched into L2 well ahead (-> 267): with 128 KB of

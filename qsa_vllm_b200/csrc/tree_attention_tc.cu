@@ -19,10 +19,10 @@
 // Roles: warp 0 loads query, key and value tiles page by page with TMA into a
 // ring; one lane of warp 1 issues all tensor-core work; warps 2-5 and 6-9
 // are the softmax warpgroups, one thread per row of S (a TMEM lane).
-//  * The maximum that p is taken against moves only when it would let p pass
-//    2^8 (rescaling O costs a round trip through TMEM); sums stay below 2^24
-//    of it, well inside fp32, and p keeps its relative precision in bf16 and
-//    fp16.
+//  * The maximum that p is taken against moves only when a tile's p add up to
+//    more than 2^8 (rescaling O costs a round trip through TMEM), which also
+//    bounds each of them: p keeps its relative precision in bf16 and fp16, and
+//    no tile but a piece's first needs its maximum taken.
 //  * P overwrites its S tile, two values to a column.
 //  * Tiles that lie wholly before the drafted tokens on mapped pages carry no
 //    mask.  In the others each row forms its 128 mask bits, values of tokens
@@ -37,16 +37,18 @@
 // tokens with a row tile each, so that the keys and values one brings from
 // memory the others find in L2.
 //
-// Measured on a B200.  64 requests of 8k-32k tokens, trees of 16, 32 query
-// heads over 4 KV heads of 128 (memory-bound): 475 us, 5.7 TB/s of keys and
-// values, 87% of a copy's rate; without the softmax arithmetic 427 us.  8
-// requests of 131072 tokens, trees of 64 (twice 128 rows a KV head and CTA
-// pair): 980 us, 1.1 PFLOP/s at the 1.5 GHz that the power limit leaves; its
-// products alone take 785 us.  There a CTA's two row tiles spend 3400 cycles
-// on a tile of tokens: 2048 of the tensor core, 2400 of the two softmax passes
-// (half of that the special-function unit), which overlap in part, as a row
-// tile's next scores wait for its P V: TMEM holds two S and two O tiles and
-// no more.
+// Measured on a B200, in long runs (the power limit then holds the clocks near
+// 1.5 GHz).  64 requests of 8k-32k tokens, trees of 16, 32 query heads over 4
+// KV heads of 128 (memory-bound): 507 us, 5.3 TB/s of keys and values, 82% of
+// a copy's rate; without the softmax arithmetic 485 us.  8 requests of 131072
+// tokens, trees of 64 (twice 128 rows a KV head and CTA pair): 1110 us, 0.97
+// PFLOP/s; without the softmax arithmetic 916.  There a CTA's two row tiles
+// spend 3400 cycles on a tile of tokens: 2048 of the tensor core, 2400 of the
+// two softmax passes (2048 of it the special-function unit), which overlap in
+// part, as a row tile's next scores wait for its P V: TMEM holds two S and two
+// O tiles and no more.  Taking every tile's maximum beside its exponentials
+// cost 1147 and 522 us; exponentials by a polynomial on the multiply-add pipe,
+// a quarter of them, gained nothing (issue slots run out first).
 //
 // Every wait is bounded; on expiry the error word is set, the CTA stops
 // issuing work, waits (bounded) for its own copies and products, frees its
@@ -71,7 +73,7 @@ constexpr int kTreeThreads = 320;
 constexpr int kTile = 128;          // tokens per tile, and rows per row tile
 constexpr int kMetaRing = 8;
 constexpr int kTmemCols = 512;      // S0 S1 O0 O1
-constexpr float kSlack = 8.0f;      // log2 of the largest p
+constexpr float kMostSum = 256.0f;  // of a tile's p against a maximum that stays
 constexpr int64_t kMinTiles = 2;    // token tiles that a CTA takes at least
 
 // What the merge kernel learns of a range that begins inside a unit.
@@ -103,7 +105,7 @@ struct TreeCfg {
   static constexpr int kStreams = DUAL ? 2 : 1;       // row tiles
   // Up to 64 rows of a single row tile, shifted apart: room for the second
   // warpgroup's O.  Not for head dim 128, where it would cost a sixth of the
-  // ring (475 -> 550 us for the first shape above).
+  // ring (475 -> 550 us for the first shape above, in short runs).
   static constexpr bool kApart = !DUAL && D == 64;
   static constexpr int kXchgBytes = kApart ? 64 * D * 4 : 16;
   static constexpr int kFit =
@@ -113,7 +115,7 @@ struct TreeCfg {
   // tiles the product with the values of tile j comes between the scores of
   // tiles j + 1 and j + 2; loaded beside their keys they would hold their
   // places, and those of the keys behind them, for two tiles (487 us instead
-  // of 475 for the first shape above; two tiles later they are no better).
+  // of 475 for the first shape above, in short runs; two tiles later they are no better).
   static constexpr int kLag = DUAL ? 0 : 1;
   static __device__ __forceinline__ int key_pos(int n) { return n < kLag ? n : 2 * n - kLag; }
   static __device__ __forceinline__ int value_pos(int n) { return 2 * n + kLag + 1; }
@@ -290,18 +292,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// One pass over a row's 128 scores: their maximum (returned), and against m
-// their exponentials, as 16-bit pairs in pk, and the sum of those in 32 bits.
-// The special-function unit takes 8 cycles for a warp's exponential, 1024 for
-// the row, the rest about half of that: a pass alone on its scheduler takes
-// 1550 cycles, two at once 2400.
+// A row's highest score.
+__device__ __forceinline__ float row_max(uint32_t ts) {
+  float high = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t s[32];
+    tmem_ld32(ts + k * 32, s);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; e += 2)
+      high = max3(high, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+  }
+  return high;
+}
+
+// The exponentials of a row's 128 scores against m, as 16-bit pairs in pk;
+// returns their sum in 32 bits.  The special-function unit takes 8 cycles for
+// a warp's exponential, 1024 for the row; the rest is issued beside it.
 template <bool F16>
-__device__ __forceinline__ float score_pass(uint32_t ts, float c, float m, uint32_t* pk,
-                                            float2& sum) {
+__device__ __forceinline__ float score_pass(uint32_t ts, float c, float m, uint32_t* pk) {
   const float shift = m == -INFINITY ? 0.0f : -m * c;
   const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
-  float high = -INFINITY;
-  sum = make_float2(0.0f, 0.0f);
+  float2 sum = make_float2(0.0f, 0.0f);
   uint32_t s[2][32];
   tmem_ld32(ts, s[0]);
 #pragma unroll
@@ -311,16 +324,14 @@ __device__ __forceinline__ float score_pass(uint32_t ts, float c, float m, uint3
     uint32_t* v = s[k & 1];
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
-      const float a = __uint_as_float(v[e]), b = __uint_as_float(v[e + 1]);
-      float2 x = fma2(make_float2(a, b), c2, shift2);
+      float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2, shift2);
       x.x = fast_exp2(x.x);
       x.y = fast_exp2(x.y);
-      high = max3(high, a, b);
       sum = add2(sum, x);
       pk[k * 16 + e / 2] = pack2<F16>(x.x, x.y);
     }
   }
-  return high;
+  return sum.x + sum.y;
 }
 
 // Clears the bits of tile t's columns that row i0 + local of the request does
@@ -812,28 +823,29 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
             ++vsyncs;
           }
         }
-        // One pass over the scores takes their maximum and, against the
-        // maximum so far, their exponentials.  Where the new maximum lies too
-        // far above (always in a piece's first tile, rarely later) it becomes
-        // the one to take them against, and the pass is made again: S is
-        // still whole, as P is only written behind this loop.
         if (!busy) {  // P of rows that are none may be anything
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.p_ready[st]);
           continue;
         }
+        // A piece's first tile gives the maximum that exponentials are taken
+        // against.  Later tiles take theirs against it at once: only where
+        // their sum passes kMostSum (no exponential can, then), or the row has
+        // seen nothing so far, is the tile's own maximum looked up, and the
+        // pass made again against that: S is still whole, as P is only
+        // written behind it.
+        if (fresh) m = row_max(ts);
         uint32_t pk[kTile / 2];
-        float2 sum;
-        for (bool settled = false;;) {
-          const float high = score_pass<F16>(ts, c, m, pk, sum);
-          if (settled) break;
-          const bool move =
-              fresh || (high > m && (m == -INFINITY || (high - m) * c > kSlack));
-          if (!__any_sync(0xffffffffu, move)) break;
-          settled = true;
-          if (!fresh) {
+        float sum = score_pass<F16>(ts, c, m, pk);
+        if (!fresh) {
+          const bool move = m == -INFINITY || sum > kMostSum;
+          if (__any_sync(0xffffffffu, move)) {
+            const float top = row_max(ts);  // of the whole warp's rows, as loads go
+            const float high = move ? fmaxf(top, m) : m;
             // the products so far are done: this S was issued behind them
-            const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : fast_exp2((m - high) * c);
+            const float f = !move || high == m ? 1.0f
+                            : m == -INFINITY   ? 0.0f
+                                               : fast_exp2((m - high) * c);
             l *= f;
 #pragma unroll
             for (int k = 0; k < D; k += 16) {
@@ -844,13 +856,14 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tmem_st16(to + k, o);
             }
+            m = high;
+            sum = score_pass<F16>(ts, c, m, pk);
           }
-          if (move) m = high;
-          fresh = false;
         }
+        fresh = false;
         tmem_st32(ts, pk);
         tmem_st32(ts + 32, pk + 32);
-        l += sum.x + sum.y;
+        l += sum;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
