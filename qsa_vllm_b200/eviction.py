@@ -126,9 +126,9 @@ def cache_compact(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: tor
     k_cache / v_cache: ``[blocks, page, H_kv, d]``; block_table, out_table: int32 ``[B, width]``;
     indices: int32 ``[B, n]`` or ``[B, H_kv, n]``, negative entries move nothing; starts: int32
     ``[B]`` (0 where None).  Without ``out_table`` the move is in place: lists ascend, no token
-    moves to a higher number, and no two requests share a page.  With it, destinations are pages that the call does not
-    read.  Entries outside the tables or on unmapped pages are skipped and set the device error
-    word."""
+    moves to a higher number, and no two requests share a page.  With it, destinations are pages
+    that the call does not read.  Entries outside the tables or on unmapped pages are skipped and
+    set the device error word."""
     what = "cache_compact"
     caches = _caches(what, k_cache, v_cache)
     dev = k_cache.get_device()
@@ -169,7 +169,8 @@ def cache_evict(weights: torch.Tensor, seq_lens: torch.Tensor, block_table: torc
     0 or above, as ``accumulate_attention_weights`` leaves them; seq_lens: int32 ``[B]`` cached
     tokens (at most ``capacity`` count), not written.  Kept are the first ``sinks`` tokens, the
     last ``recent`` and the heaviest of the others, ties to the lowest token.  Their K/V rows
-    move to tokens ``0 .. budget - 1`` in place, or to the pages of ``out_table``; their weights
+    move to tokens ``0 .. budget - 1`` in place (no two requests may share a page then), or to
+    the pages of ``out_table``, which the call does not read; their weights
     to the front of ``weights_out`` (``weights`` itself where None), with zeros up to the old
     length.  kept: int32 ``[B, heads of weights, budget]``, the old token numbers, -1 behind the
     last; lengths: int32 ``[B]``."""
