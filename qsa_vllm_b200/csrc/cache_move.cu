@@ -148,10 +148,10 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(MoveParams p) {
 }
 
 // New lengths, and the number of tokens each list head chooses from (0 where
-// nothing is evicted).  Written before the next kernel may start: the top-k
-// reads its rows' lengths before its own wait.
+// nothing is evicted), which the top-k reads behind its wait for this kernel.
 __global__ void evict_lengths_kernel(MoveParams p, int32_t* lengths_out, int32_t* middle) {
   pdl_wait();
+  pdl_trigger();
   const int n = blockIdx.x * blockDim.x + threadIdx.x;
   if (n < p.requests * p.list_heads) {
     int b, h;
@@ -160,8 +160,6 @@ __global__ void evict_lengths_kernel(MoveParams p, int32_t* lengths_out, int32_t
     middle[n] = seq > p.budget ? seq - p.sinks - p.recent : 0;
     if (h == 0) lengths_out[b] = min(seq, p.budget);
   }
-  __threadfence();
-  pdl_trigger();
 }
 
 template <typename U>
@@ -213,6 +211,7 @@ cudaError_t launch_cache_evict(const MoveParams& p, int32_t* lengths_out, int32_
     t.rows = lists;
     t.width = p.capacity - p.sinks - p.recent;
     t.lengths = middle;
+    t.lengths_behind_wait = 1;
     t.output = chosen;
     t.out_row_stride = p.chosen_width;
     t.out_col_stride = 1;

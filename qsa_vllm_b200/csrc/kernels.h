@@ -16,6 +16,7 @@ struct TopkParams {
   int64_t score_row_stride;
   int rows, width;
   const int32_t* lengths;
+  int lengths_behind_wait;  // the preceding kernel writes `lengths`
   const int64_t* positions;
   const int32_t* seq_lens;
   int num_requests;

@@ -45,6 +45,14 @@ constexpr int kBins = 2048;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSelBytes = 192 * 1024;  // selected ids of one CTA: up to 49152 blocks
 
+// Columns of a row that are chosen from.
+__device__ __forceinline__ int row_length(const TopkParams& p, int row) {
+  const int n = p.lengths != nullptr ? p.lengths[row]
+                                     : visible_of(p.positions, p.seq_lens, p.num_requests,
+                                                  p.token_to_req, p.ratio, row);
+  return min(max(n, 0), p.width);
+}
+
 // Shared-memory histogram increment.  The digits lie below the row's common
 // high bits, so lanes rarely collide on a bin.
 __device__ __forceinline__ void hist_add(int* hist, bool valid, uint32_t bin) {
@@ -121,17 +129,14 @@ __global__ void __launch_bounds__(T, 1024 / T) topk_kernel(const TopkParams p) {
   // The row's metadata (request, sequence length, position, visible count,
   // block table) is step metadata that the preceding kernel (the indexer)
   // does not write: it is read before waiting on that kernel, so these
-  // dependent loads overlap its tail.  The scores are read after the wait.
+  // dependent loads overlap its tail.  The scores are read after the wait,
+  // and so are lengths that the preceding kernel does write.
   RowMeta m{};
   if (p.expand) m = row_meta(p, row);
-  const int length =
-      min(max(p.lengths != nullptr ? p.lengths[row]
-                                   : visible_of(p.positions, p.seq_lens, p.num_requests,
-                                                p.token_to_req, p.ratio, row),
-              0),
-          p.width);
+  int length = p.lengths_behind_wait ? 0 : row_length(p, row);
   pdl_wait();
   pdl_trigger();
+  if (p.lengths_behind_wait) length = row_length(p, row);
 
   if (length <= topk || topk == 0) {
     // Every column is selected (topk.cu:187-191), or none is asked for; no
@@ -376,16 +381,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) topk_warp_kernel(const Topk
   // row metadata before the wait, as in topk_kernel
   RowMeta m{};
   if (live && p.expand) m = row_meta(p, row);
-  const int length =
-      live ? min(max(p.lengths != nullptr ? p.lengths[row]
-                                          : visible_of(p.positions, p.seq_lens, p.num_requests,
-                                                       p.token_to_req, p.ratio, row),
-                     0),
-                 p.width)
-           : 0;
+  int length = live && !p.lengths_behind_wait ? row_length(p, row) : 0;
   pdl_wait();
   pdl_trigger();
   if (!live) return;
+  if (p.lengths_behind_wait) length = row_length(p, row);
 
   if (length <= topk || topk == 0) {  // all columns selected (topk.cu:187-191), or none asked
     const int n = p.expand ? max(m.complete, 0) : topk;

@@ -224,3 +224,50 @@ def test_evict_captured_again_and_again(dev):
     torch.cuda.synchronize()
     for t, s in zip((k, v, w, seq), want):
         assert torch.equal(t, s)
+
+
+@pytest.mark.parametrize("requests,hkv,ctx,budget", [
+    (300, 2, 96, 40),       # 600 lists: the lengths come from several blocks of several warps
+    (61, 8, 2300, 700),     # 488 lists, a wider form of the selection
+    (1000, 4, 2000, 64),    # a warp for each list
+    (40, 1, 9000, 1000),    # a cluster for each list
+])
+def test_evict_many_lists_of_different_lengths(dev, requests, hkv, ctx, budget):
+    """Each list is chosen from its own request's length, call after call in one workspace: the
+    lengths of a call must be neither the one's before nor what the workspace held."""
+    from qsa_vllm_b200 import _lib
+    from qsa_vllm_b200.eviction import cache_evict, cache_evict_workspace_bytes
+    g = torch.Generator().manual_seed(requests + ctx)
+    kv = torch.randn(32, 16, hkv, 16, generator=g).to(BF16).to(dev)
+    k, v = kv[..., :8], kv[..., 8:]
+    table = torch.randint(0, 32, (requests, -(-ctx // 16)), generator=g).to(torch.int32).to(dev)
+    other = torch.full((requests, 1), -1, dtype=torch.int32, device=dev)
+    need = cache_evict_workspace_bytes(requests, hkv, budget, 3, 5)
+    workspace = torch.full((need,), 0x7f, dtype=torch.uint8, device=dev)
+    calls = []
+    for n in range(3):  # queued one behind another, read afterwards
+        seq = torch.randint(0, ctx + 1, (requests,), generator=g).to(torch.int32)
+        w = torch.rand(requests, hkv, ctx, generator=g)
+        kept = torch.empty(requests, hkv, budget, dtype=torch.int32, device=dev)
+        lens, weights, out = seq.to(dev), w.to(dev), torch.zeros_like(w, device=dev)
+        calls.append((seq, w, kept, lens, weights, out))
+    torch.cuda.synchronize()
+    keep_k = k.clone()
+    for seq, w, kept, lens, weights, out in calls:
+        # destinations without pages: no row finds a place, which is reported
+        cache_evict(weights, lens, table, k, v, budget, sinks=3, recent=5, out_table=other,
+                    weights_out=out, kept=kept, workspace=workspace)
+    torch.cuda.synchronize()
+    assert torch.equal(k, keep_k) and _lib.device_error_poll() == 2
+    for seq, w, kept, lens, weights, out in calls:
+        t = torch.arange(ctx)
+        n = seq.long()[:, None, None]
+        rank = torch.where((t < 3) | (t >= n - 5), 2.0, w)
+        rank = torch.where(t < n, rank, -1.0)
+        order = rank.sort(dim=-1, descending=True, stable=True).indices[..., :budget]
+        here = torch.arange(budget) < n.clamp(max=budget)
+        want = torch.where(here, order, ctx).sort(-1).values
+        want = torch.where(here, want, -1)
+        assert torch.equal(kept.cpu().long(), want)
+        w_want = torch.where(here, w.gather(2, want.clamp(min=0)), 0.0)
+        assert torch.equal(out.cpu()[..., :budget], w_want) and not out[..., budget:].any()
