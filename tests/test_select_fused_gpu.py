@@ -210,3 +210,31 @@ def test_select_decode_declines_shapes_outside_its_range(dev):
 def test_select_decode_no_device_errors(dev):
     from qsa_vllm_b200 import _lib
     assert _lib.device_error_poll() == 0
+
+
+@pytest.mark.parametrize("rows", [37, 600])
+def test_counts_of_the_kernel_before_are_all_there(dev, rows):
+    """A selection that directly follows the kernel that computes its rows' counts, again and
+    again with other counts, in memory that held the counts of the time before."""
+    from qsa_vllm_b200.indexer import compute_visible_blocks
+    from qsa_vllm_b200.topk import topk
+    g = torch.Generator().manual_seed(rows)
+    ratio, width, k = 4, 1500, 64
+    scores = torch.rand(rows, width, generator=g)
+    rising = scores.to(dev)
+    steps = []
+    for _ in range(6):
+        seq = torch.randint(1, width * ratio, (rows,), generator=g).to(torch.int32)
+        steps.append((seq, seq.to(dev), (seq.long() - 1).to(dev),
+                      torch.empty(rows, k, dtype=torch.int32, device=dev)))
+    t2r = torch.arange(rows, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    for seq, lens, pos, out in steps:
+        topk(rising, compute_visible_blocks(pos, lens, t2r, ratio), out)
+    for seq, lens, pos, out in steps:
+        n = (seq.long() // ratio)[:, None]
+        rank = torch.where(torch.arange(width) < n, scores, -1.0)
+        want = rank.sort(dim=-1, descending=True, stable=True).indices[:, :k]
+        here = torch.arange(k) < n
+        want = torch.where(here, want, width).sort(-1).values
+        assert torch.equal(out.cpu().long(), torch.where(here, want, -1))
