@@ -121,8 +121,8 @@ enum {
  * min((positions[r] + 1) // ratio, sequence_lengths[req] // ratio) (0 for an
  * unmapped row), as qsa_visible_blocks computes it.
  * Limits (QSA_ERR_UNSUPPORTED beyond them): score_width up to 524288 columns
- * (16-CTA clusters of 1024 threads x 32 keys), K up to 49152 blocks (one
- * row's selection in 192 KB of shared memory); the same for qsa_topk.
+ * (16-CTA clusters of 1024 threads x 32 keys), K up to 49152 blocks; the same
+ * for qsa_topk.
  */
 QSA_API int qsa_topk_expand(const float* scores, int64_t score_row_stride, int32_t rows,
                     int32_t score_width, const int32_t* lengths, const int64_t* positions,
@@ -538,8 +538,8 @@ QSA_API size_t qsa_cache_evict_workspace_bytes(int32_t num_requests, int32_t lis
  * weights_out unless it is weights may overlap what the call reads.
  * weights: fp32 [num_requests, list_heads, capacity], unit token stride,
  * (request, head) rows evenly spaced; list_heads = num_kv_heads, or 1 for a
- * list shared by all heads.  Up to topk limits (see qsa_topk): capacity -
- * sinks - recent <= 524288, budget - sinks - recent <= 49152.
+ * list shared by all heads.  Where there is a choice to make (capacity > budget
+ * > sinks + recent), capacity - sinks - recent is at most 524288.
  */
 QSA_API int qsa_cache_evict(
     const float* weights, int64_t weights_request_stride, int64_t weights_head_stride,

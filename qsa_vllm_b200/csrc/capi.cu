@@ -871,9 +871,6 @@ int qsa_cache_evict(const float* weights, int64_t weights_request_stride,
     if (capacity - sinks - recent > topk_max_width())
       return fail(QSA_ERR_UNSUPPORTED, "%s: %d tokens to choose from exceed %d", who,
                   capacity - sinks - recent, topk_max_width());
-    if (chosen > topk_max_blocks())
-      return fail(QSA_ERR_UNSUPPORTED, "%s: %d tokens to choose exceed %d", who, chosen,
-                  topk_max_blocks());
     if ((num_requests > 1 || list_heads > 1) && row_stride < capacity)
       return fail(QSA_ERR_INVALID, "%s: weights row stride %lld < %d", who, (long long)row_stride,
                   capacity);

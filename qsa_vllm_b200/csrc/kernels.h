@@ -41,7 +41,7 @@ struct TopkParams {
 cudaError_t launch_topk(const TopkParams& p, cudaStream_t stream, int* plan_cluster);
 // Largest score width the shared-memory-resident select supports.
 int topk_max_width();
-// Largest top-k (in blocks) one row's selection can hold in shared memory.
+// Largest top-k (in blocks) that the selection entry points take.
 int topk_max_blocks();
 
 // --------------------------------------------------------------- indexer

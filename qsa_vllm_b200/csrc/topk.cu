@@ -43,7 +43,7 @@ namespace {
 constexpr int kThreads = 1024;  // widest CTA (rows above 4096 keys and clusters)
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 16;
-constexpr int kMaxSelBytes = 192 * 1024;  // selected ids of one CTA: up to 49152 blocks
+constexpr int kMaxBlocks = 49152;  // top-k of the public selection entry points
 
 // Columns of a row that are chosen from.
 __device__ __forceinline__ int row_length(const TopkParams& p, int row) {
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(T, 1024 / T) topk_kernel(const TopkParams p) {
   constexpr int kChunks = V / 4;
   constexpr int kWarps = T / 32;
   constexpr int kPer = kBins / T > 0 ? kBins / T : 1;  // most bins one thread ranks
-  extern __shared__ int sel[];  // selected column ids of this CTA, by rank (topk entries)
+  extern __shared__ int sel[];  // selected column ids of this CTA, by rank
   __shared__ int hist[2][kBins];
   __shared__ int warp_tmp[kWarps * kChunks * 2];
   __shared__ uint32_t s_minmax[2][kWarps];
@@ -544,10 +544,12 @@ int pow2_ceil(int x) {
 
 template <int T, int V>
 cudaError_t launch_v(TopkParams p, int C, cudaStream_t stream) {
-  const int smem = std::max(p.topk, 1) * static_cast<int>(sizeof(int));
-  if (smem > kMaxSelBytes) return cudaErrorInvalidValue;
+  // selected ids of one CTA: no more than its slice holds keys
+  constexpr int kSlice = T * V;
+  const size_t smem = std::min(std::max(p.topk, 1), kSlice) * sizeof(int);
   cudaError_t e0 = set_attr_once(reinterpret_cast<const void*>(topk_kernel<T, V>),
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSelBytes);
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kSlice * static_cast<int>(sizeof(int)));
   if (e0 != cudaSuccess) return e0;
   if (C > 8) {
     cudaError_t e = set_attr_once(reinterpret_cast<const void*>(topk_kernel<T, V>),
@@ -556,15 +558,14 @@ cudaError_t launch_v(TopkParams p, int C, cudaStream_t stream) {
   }
   return count_launches(launch_kernel(
       topk_kernel<T, V>, dim3(static_cast<unsigned>(C) * static_cast<unsigned>(p.rows)),
-      dim3(T), static_cast<size_t>(std::max(p.topk, 1)) * sizeof(int), stream,
-      static_cast<unsigned>(C), p));
+      dim3(T), smem, stream, static_cast<unsigned>(C), p));
 }
 
 }  // namespace
 
 int topk_max_width() { return kMaxCluster * kThreads * 32; }
 
-int topk_max_blocks() { return kMaxSelBytes / static_cast<int>(sizeof(int)); }
+int topk_max_blocks() { return kMaxBlocks; }
 
 cudaError_t launch_topk(const TopkParams& p0, cudaStream_t stream, int* plan_cluster) {
   TopkParams p = p0;

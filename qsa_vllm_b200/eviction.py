@@ -173,7 +173,12 @@ def cache_evict(weights: torch.Tensor, seq_lens: torch.Tensor, block_table: torc
     the pages of ``out_table``, which the call does not read; their weights
     to the front of ``weights_out`` (``weights`` itself where None), with zeros up to the old
     length.  kept: int32 ``[B, heads of weights, budget]``, the old token numbers, -1 behind the
-    last; lengths: int32 ``[B]``."""
+    last; lengths: int32 ``[B]``.
+
+    Refused with :class:`QSAError`: weights whose (request, head) rows are not evenly spaced (a
+    slice of the heads of more), and more than 524288 tokens to choose from (``capacity - sinks
+    - recent``, where the budget is below the capacity).  Kept tokens outside a table or on
+    unmapped pages are not moved and set the device error word."""
     what = "cache_evict"
     caches = _caches(what, k_cache, v_cache)
     dev = k_cache.get_device()

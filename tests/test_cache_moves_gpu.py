@@ -271,3 +271,42 @@ def test_evict_many_lists_of_different_lengths(dev, requests, hkv, ctx, budget):
         assert torch.equal(kept.cpu().long(), want)
         w_want = torch.where(here, w.gather(2, want.clamp(min=0)), 0.0)
         assert torch.equal(out.cpu()[..., :budget], w_want) and not out[..., budget:].any()
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("lengths,budget,sinks,recent", [
+    ([70000, 55001, 64], 55000, 0, 0),
+    ([65536], 65535, 0, 0),                    # one token goes
+    ([300000, 299000], 200000, 16, 1024),
+    ([524288 + 9, 524288], 500000, 4, 5),      # the most there is to choose from
+])
+def test_evict_large_budgets(dev, in_place, lengths, budget, sinks, recent):
+    from qsa_vllm_b200 import _lib
+    from qsa_vllm_b200.eviction import cache_evict
+    g = torch.Generator().manual_seed(budget)
+    requests, capacity = len(lengths), max(lengths)
+    k, v, table, other = pool(g, dev, requests, capacity, 64, 1, 8, BF16,
+                              0 if in_place else -(-budget // 64))
+    w = torch.randint(0, 1 << 16, (requests, 1, capacity), generator=g).float()
+    w[torch.rand(w.shape, generator=g) < 0.2] = 0
+    keep = [torch.tensor(chosen(w[b, 0], n, budget, sinks, recent)) for b, n in enumerate(lengths)]
+    k0, v0, table0 = k.cpu(), v.cpu(), table.cpu().long()
+    to = table0 if in_place else other.cpu().long()
+    k1, v1 = k0.clone(), v0.clone()
+    for b, at in enumerate(keep):
+        t = torch.arange(at.numel())
+        k1[to[b][t // 64], t % 64], v1[to[b][t // 64], t % 64] = \
+            k0[table0[b][at // 64], at % 64], v0[table0[b][at // 64], at % 64]
+    weights = w.to(dev)
+    out = None if in_place else torch.zeros_like(weights)
+    kept, count = cache_evict(weights, torch.tensor(lengths, dtype=torch.int32, device=dev), table,
+                              k, v, budget, sinks=sinks, recent=recent,
+                              out_table=None if in_place else other, weights_out=out)
+    got = (weights if in_place else out).cpu()
+    for b, at in enumerate(keep):
+        n = at.numel()
+        assert torch.equal(kept[b, 0, :n].cpu().long(), at) and (kept[b, 0, n:] == -1).all()
+        assert count[b] == n and torch.equal(got[b, 0, :n], w[b, 0, at])
+        assert not got[b, 0, n:lengths[b]].any()
+    assert torch.equal(k.cpu(), k1) and torch.equal(v.cpu(), v1)
+    assert _lib.device_error_poll() == 0

@@ -264,3 +264,14 @@ def test_tree_c_abi_refusals():
     for bad in ((0, 2, 8, 2, 128, 2), (4, 0, 8, 2, 128, 2), (4, 2, 7, 2, 128, 2), (4, 2, 8, 2, 128, 0),
                 (4, 2, 8, 2, 72, 2)):
         assert lib.qsa_tree_attention_workspace_bytes(*bad) == 0
+
+
+def test_evict_takes_any_budget():
+    """Budgets past what the selection's own entry points take are not refused (a missing
+    workspace is, behind every check of sizes)."""
+    from qsa_vllm_b200 import _lib
+    lib = _lib.load_library()
+    for cap, budget in (65536, 60000), (524288, 524287), (1 << 20, 1 << 20):
+        assert lib.qsa_cache_evict(4096, cap, cap, 1, cap, 4096, 1, budget, 0, 0, 4096, 64, 64, 64,
+                                   4096, 64, 64, 64, 8, 16, 1, 64, 0, 4096, 4, 4, None, 0, 0, 4096,
+                                   cap, cap, 4096, 4096, None, 0, None) == 3, (cap, budget)
