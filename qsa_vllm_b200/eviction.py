@@ -24,6 +24,7 @@ from .qsa import aligned_head_rows
 from .tree_attention import check_lse, check_tree_arguments
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_NO_COLUMNS = 16
 
 
 def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple:
@@ -62,8 +63,10 @@ def _tables(what: str, dev: int, block_table: torch.Tensor, out_table) -> tuple:
     if out_table is None:
         return block_table.data_ptr(), block_table.stride(0), width, None, 0, 0
     _int32(what, "out_table", out_table, dev, requests, None)
-    return (block_table.data_ptr(), block_table.stride(0), width, out_table.data_ptr(),
-            out_table.stride(0), out_table.shape[1])
+    # A table without columns has no storage, but it is not the in-place move that a null pointer
+    # means: any other pointer does, as none of it is read.
+    return (block_table.data_ptr(), block_table.stride(0), width,
+            out_table.data_ptr() or _NO_COLUMNS, out_table.stride(0), out_table.shape[1])
 
 
 def accumulate_attention_weights(

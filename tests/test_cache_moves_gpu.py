@@ -310,3 +310,15 @@ def test_evict_large_budgets(dev, in_place, lengths, budget, sinks, recent):
         assert not got[b, 0, n:lengths[b]].any()
     assert torch.equal(k.cpu(), k1) and torch.equal(v.cpu(), v1)
     assert _lib.device_error_poll() == 0
+
+
+def test_compact_to_a_table_without_columns_moves_nothing(dev):
+    from qsa_vllm_b200 import _lib
+    from qsa_vllm_b200.eviction import cache_compact
+    g = torch.Generator().manual_seed(4)
+    k, v, table, _ = pool(g, dev, 2, 64, 16, 2, 64, BF16)
+    k0, v0 = k.clone(), v.clone()
+    idx = torch.tensor([[5, 9], [-1, 7]], dtype=torch.int32, device=dev)
+    cache_compact(k, v, table, idx, out_table=table[:, :0])
+    assert _lib.device_error_poll() == 2
+    assert torch.equal(k, k0) and torch.equal(v, v0)

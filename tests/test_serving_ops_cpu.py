@@ -275,3 +275,12 @@ def test_evict_takes_any_budget():
         assert lib.qsa_cache_evict(4096, cap, cap, 1, cap, 4096, 1, budget, 0, 0, 4096, 64, 64, 64,
                                    4096, 64, 64, 64, 8, 16, 1, 64, 0, 4096, 4, 4, None, 0, 0, 4096,
                                    cap, cap, 4096, 4096, None, 0, None) == 3, (cap, budget)
+
+
+def test_a_table_without_columns_is_not_in_place():
+    from qsa_vllm_b200.eviction import _tables
+    table = torch.zeros(2, 4, dtype=torch.int32)
+    for empty in table[:, :0], torch.zeros(2, 0, dtype=torch.int32):
+        got = _tables("cache_compact", -1, table, empty)
+        assert got[3] and got[3] != got[0] and got[5] == 0
+    assert _tables("cache_compact", -1, table, None)[3] is None
