@@ -8,9 +8,10 @@
 // head) pairs of the request the N side, up to 256 at a time, and each
 // thread of the epilogue adds up the columns of its own token:
 //   S[128 x N] = K Q^T     (A, B from shared memory, D in TMEM, two in turn)
-// Only rows that count (factor not 0, log-sum-exp not -inf) are gathered into
-// the N side.  Requests with more pairs than 256 take several passes over the
-// tile range, one after another (all epilogue warps meet between them).
+// Only rows that count (factor not 0, some head's log-sum-exp not -inf) are
+// gathered into the N side.  Requests with more pairs than 256 take several
+// passes over the tile range, one after another (all epilogue warps meet
+// between them).
 //
 // Bound by the keys' way from memory: a tile is 32 KB (head dim 128), its
 // products N/2 cycles of the tensor core's 8192 flops, its exponentials
@@ -104,6 +105,16 @@ __device__ __forceinline__ int weight_tiles(const TreeParams& p, int b) {
 // TMEM buffer of the j-th tile of a pass.
 __device__ __forceinline__ int weights_buffer(int j, int pairs) {
   return pairs <= 128 ? j & 3 : (j & 1) * 2;
+}
+
+// Whether a packed row counts: a factor other than 0, and a log-sum-exp of KV
+// head h other than -inf (its first, almost always).
+__device__ __forceinline__ bool weights_row_counts(const TreeParams& p, int64_t row, int h) {
+  if (p.row_factors != nullptr && p.row_factors[row * p.factor_stride] == 0.0f) return false;
+  const float* lse = p.lse + row * p.lse_row_stride + h * p.group;
+  for (int g = 0; g < p.group; ++g)
+    if (lse[g] != -INFINITY) return true;
+  return false;
 }
 
 template <int D, bool F16>
@@ -242,12 +253,7 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
       int counted = 0;
       for (int i0 = 0; i0 < r.count; i0 += 32) {
         const int i = i0 + lane;
-        bool in = false;
-        if (i < r.count) {
-          const int64_t row = r.row0 + i;
-          in = (p.row_factors == nullptr || p.row_factors[row * p.factor_stride] != 0.0f) &&
-               p.lse[row * p.lse_row_stride + h * p.group] != -INFINITY;
-        }
+        const bool in = i < r.count && weights_row_counts(p, r.row0 + i, h);
         counted += __popc(__ballot_sync(0xffffffffu, in));
       }
       const int rows_per_pass = kPairs / p.group;
@@ -375,12 +381,7 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
           int got = 0, i0 = from, next = r.count;
           for (; i0 < r.count; i0 += 32) {
             const int i = i0 + lane;
-            bool in = false;
-            if (i < r.count) {
-              const int64_t row = r.row0 + i;
-              in = (p.row_factors == nullptr || p.row_factors[row * p.factor_stride] != 0.0f) &&
-                   p.lse[row * p.lse_row_stride + pc.h * p.group] != -INFINITY;
-            }
+            const bool in = i < r.count && weights_row_counts(p, r.row0 + i, pc.h);
             const uint32_t bits = __ballot_sync(0xffffffffu, in);
             const int at = got + __popc(bits & ((1u << lane) - 1));
             if (in && at < rows_per_pass) sm.list[at] = i;
@@ -443,7 +444,7 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
             const int64_t row = r.row0 + i;
             l = p.lse[row * p.lse_row_stride + pc.h * p.group + head] * -1.4426950408889634f;
             f = p.row_factors == nullptr ? 1.0f : p.row_factors[row * p.factor_stride];
-            if (l == INFINITY) l = -INFINITY;  // a head that saw nothing
+            if (l == INFINITY) f = 0.0f;  // a head that saw nothing, in a row that counts
             fold = f > 0.0f && f < INFINITY && l == l;
             if (fold) {
               l += log2f(f);
@@ -553,13 +554,14 @@ attention_weights_kernel(const __grid_constant__ TreeParams p,
                   acc[0] = add2(acc[0], x);
                   acc[1] = add2(acc[1], y);
                 }
-              } else {  // a factor below 0, infinite or NaN, or a NaN log-sum-exp
+              } else {
+                // a factor below 0, infinite or NaN, a NaN log-sum-exp, or a
+                // head that saw nothing (factor 0)
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                  const float x =
-                      sm.factor[k + e] *
-                      fast_exp2(fmaf(__uint_as_float(v[e]), c, sm.shift[k + e]));
-                  acc[e & 1].x += (sees >> e) & 1 ? x : 0.0f;
+                  const float f = sm.factor[k + e];
+                  const float x = f * fast_exp2(fmaf(__uint_as_float(v[e]), c, sm.shift[k + e]));
+                  acc[e & 1].x += (sees >> e) & 1 && f != 0.0f ? x : 0.0f;
                 }
               }
             }

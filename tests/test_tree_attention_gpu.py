@@ -416,3 +416,24 @@ def test_weights_captured_add_up(dev):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.allclose(w, 2 * once, rtol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("page,d", [(16, 128), (64, 64), (5, 64)])
+@pytest.mark.parametrize("factored", [False, True])
+def test_weights_of_rows_with_heads_left_out(dev, page, d, factored):
+    """A head whose log-sum-exp is -inf gives nothing, whatever it holds; the row's other heads
+    give what they give, whichever of them it is.  More rows than a pass takes."""
+    c = tc.make(34, [700, 260, 90], [70, 3, 5], 8, 2, d, page, BF16, "tree", dev, poison=False)
+    _, lse = call(c)
+    lse[:, 0] = -torch.inf           # the first head of the first group, of every row
+    lse[3:60:7, 4:7] = -torch.inf    # all but the last head of the second
+    lse[5] = lse[71] = -torch.inf    # whole rows
+    lse[9, 5] = -torch.inf
+    c["q"][9, 5] = float("nan")
+    factors = torch.linspace(0.25, 2, 78).to(dev) if factored else None
+    if factored:
+        factors[8::9] = 0
+    got = accumulate(c, lse, torch.ones(3, 2, 700, device=dev), row_factors=factors)
+    clean = dict(c, q=torch.nan_to_num(c["q"], 0.0))
+    want, tol = tc.weights(clean, lse, torch.ones(3, 2, 700), factors)
+    tc.compare(got, want, tol, "weights")
