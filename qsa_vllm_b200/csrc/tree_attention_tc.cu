@@ -21,8 +21,11 @@
 // are the softmax warpgroups, one thread per row of S (a TMEM lane).
 //  * The maximum that p is taken against moves only when a tile's p add up to
 //    more than 2^8 (rescaling O costs a round trip through TMEM), which also
-//    bounds each of them: p keeps its relative precision in bf16 and fp16, and
-//    no tile but a piece's first needs its maximum taken.
+//    bounds each of them, and no tile but a piece's first needs its maximum
+//    taken.  p keeps its relative precision in bf16.  fp16 has no such range:
+//    there p, and with it l and O, is taken 2^7 times as large (at most 2^15),
+//    so that its last bit is 2^-31 of the maximum, and what 2^20 tokens lose
+//    below it at most half an output's rounding.
 //  * P overwrites its S tile, two values to a column.
 //  * Tiles that lie wholly before the drafted tokens on mapped pages carry no
 //    mask.  In the others each row forms its 128 mask bits, values of tokens
@@ -74,6 +77,7 @@ constexpr int kTile = 128;          // tokens per tile, and rows per row tile
 constexpr int kMetaRing = 8;
 constexpr int kTmemCols = 512;      // S0 S1 O0 O1
 constexpr float kMostSum = 256.0f;  // of a tile's p against a maximum that stays
+template <bool F16> constexpr float kLift = F16 ? 7.0f : 0.0f;  // log2 of the factor on p
 constexpr int64_t kMinTiles = 2;    // token tiles that a CTA takes at least
 
 // What the merge kernel learns of a range that begins inside a unit.
@@ -307,12 +311,12 @@ __device__ __forceinline__ float row_max(uint32_t ts) {
   return high;
 }
 
-// The exponentials of a row's 128 scores against m, as 16-bit pairs in pk;
-// returns their sum in 32 bits.  The special-function unit takes 8 cycles for
+// The exponentials of a row's 128 scores against m, times 2^kLift, as 16-bit
+// pairs in pk; returns their sum in 32 bits.  The special-function unit takes 8 cycles for
 // a warp's exponential, 1024 for the row; the rest is issued beside it.
 template <bool F16>
 __device__ __forceinline__ float score_pass(uint32_t ts, float c, float m, uint32_t* pk) {
-  const float shift = m == -INFINITY ? 0.0f : -m * c;
+  const float shift = m == -INFINITY ? 0.0f : fmaf(-m, c, kLift<F16>);
   const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift);
   float2 sum = make_float2(0.0f, 0.0f);
   uint32_t s[2][32];
@@ -838,7 +842,8 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         uint32_t pk[kTile / 2];
         float sum = score_pass<F16>(ts, c, m, pk);
         if (!fresh) {
-          const bool move = m == -INFINITY || sum > kMostSum;
+          constexpr float kMost = kMostSum * (F16 ? 128.0f : 1.0f);  // 2^kLift
+          const bool move = m == -INFINITY || sum > kMost;
           if (__any_sync(0xffffffffu, move)) {
             const float top = row_max(ts);  // of the whole warp's rows, as loads go
             const float high = move ? fmaxf(top, m) : m;
@@ -916,7 +921,7 @@ tree_attention_kernel(const __grid_constant__ TreeParams p, const __grid_constan
         const bool live = busy && local < R && i < r.count;
         const bool whole = tiles == pc.tiles;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const float lse2 = l == 0.0f ? -INFINITY : m * c + log2f(l);
+        const float lse2 = l == 0.0f ? -INFINITY : m * c + (log2f(l) - kLift<F16>);
         const int64_t packed = r.row0 + i;
         const int q_head = pc.h * p.group + head;
         const int64_t part_row =

@@ -437,3 +437,44 @@ def test_weights_of_rows_with_heads_left_out(dev, page, d, factored):
     clean = dict(c, q=torch.nan_to_num(c["q"], 0.0))
     want, tol = tc.weights(clean, lse, torch.ones(3, 2, 700), factors)
     tc.compare(got, want, tol, "weights")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d,count,at", [(64, 1, 0), (128, 1, 0), (128, 16, 70001), (64, 40, 0),
+                                        (128, 40, 0)])
+def test_many_light_tokens_beside_a_heavy_one(dev, dtype, d, count, at):
+    """131072 tokens, of which one holds almost all of the weight: what the others give together
+    is seen although each is far below the heavy one, down to 2^-24.6.
+
+    The light tokens' values are 1 and the heavy one's 0, so an output is n p / (1 + n p).  p is
+    rounded to the type (half a step, and no finer than 2^-32 of the heavy token's in fp16);
+    sums are chains of at most n / 16 products of 16 tokens, each to 2^-23, and of 64 + n / 128
+    exponentials, each to 2^-24; the output is rounded once."""
+    n, batch, hkv, group, page = 131072, 64, 4, 8, 64
+    kv = torch.zeros(n // page, page, hkv, 2 * d, dtype=dtype, device=dev)
+    kv[at // page, at % page, :, 0] = 17.0625
+    gap = float(kv[at // page, at % page, 0, 0])  # as the type holds it
+    kv[..., d:] = 1
+    kv[at // page, at % page, :, d:] = 0
+    q = torch.zeros(batch * count, hkv * group, d, dtype=dtype, device=dev)
+    part = torch.tensor([1.0, 0.75] * (hkv * group // 2), dtype=torch.float64)
+    q[..., 0] = part.to(dtype).to(dev)
+    table = torch.arange(n // page, dtype=torch.int32, device=dev).expand(batch, -1).contiguous()
+    start = torch.arange(batch + 1, dtype=torch.int32, device=dev) * count
+    lens = torch.full((batch,), n, dtype=torch.int32, device=dev)
+    from qsa_vllm_b200.tree_attention import tree_paged_attention
+    lse = torch.empty(batch * count, hkv * group, device=dev)
+    out = tree_paged_attention(q, kv[..., :d], kv[..., d:], table, lens, start,
+                               max_query_len=count, scale=1.0, lse=lse)
+    light = (n - count + torch.arange(count).double())[:, None]  # seen, without the heavy one
+    p = (-gap * part).exp()[None]
+    want = light * p / (1 + light * p)
+    eps = torch.finfo(dtype).eps / 2
+    tiny = 2.0 ** -32 if dtype == F16 else 0.0
+    tol = want * (eps + n / 16 * 2.0 ** -23 + (64 + n / 128) * 2.0 ** -24 + 2.0 ** -18) \
+        + light * tiny / (1 + light * p)
+    tol = tol + eps * (want + tol)
+    off = (out.double().cpu().view(batch, count, -1, d) - want[..., None]).abs()
+    assert (off <= tol[..., None]).all(), (off / want[..., None]).amax((0, 1, 3))
+    z = gap * part + torch.log1p(light * p)
+    assert ((lse.double().cpu().view(batch, count, -1) - z).abs() <= 2.0 ** -13).all()
