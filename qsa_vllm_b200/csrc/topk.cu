@@ -54,7 +54,8 @@ __device__ __forceinline__ int row_length(const TopkParams& p, int row) {
 }
 
 // Shared-memory histogram increment.  The digits lie below the row's common
-// high bits, so lanes rarely collide on a bin.
+// high bits, so lanes rarely collide on a bin with scores of one magnitude;
+// with many equal keys (weights of tokens that were never attended) they do.
 __device__ __forceinline__ void hist_add(int* hist, bool valid, uint32_t bin) {
   if (valid) atomicAdd(hist + bin, 1);
 }
@@ -593,15 +594,17 @@ cudaError_t launch_topk(const TopkParams& p0, cudaStream_t stream, int* plan_clu
   // Smallest (keys per thread, cluster width) whose slices cover the row.
   int V = 8;
   int C = pow2_ceil((w + kThreads * V - 1) / (kThreads * V));
-  // Eight keys per thread finish a row soonest, as long as all rows' clusters
-  // run at once.  A CTA has its SM to itself, and a cluster lies within one
-  // group of SMs, so about 37 clusters of 4 run at once, 12 of 8 and 4 of 16;
-  // with more rows than that, 32 keys per thread in a quarter of the CTAs win
-  // (us, 8 against 32 keys: 32768 columns 32 rows 15 / 22, 64 rows 30 / 21;
-  // 65536 columns 8 rows 23 / 26, 16 rows 40 / 22; 131072 columns 4 rows
-  // 44 / 25, 32 rows 214 / 30).
-  const int at_once = C <= 4 ? num_sms() / 4 : C == 8 ? num_sms() / 12 : 0;
-  if (C > kMaxCluster || (C >= 4 && p.rows > at_once)) {
+  // Up to clusters of 8, eight keys per thread finish a row soonest, as long
+  // as all rows' clusters run at once.  A CTA has its SM to itself, and a
+  // cluster lies within one group of SMs, so about 37 clusters of 4 run at once
+  // and 12 of 8; with more rows than that, 32 keys per thread in a quarter of
+  // the CTAs win (us, 8 against 32 keys: 32768 columns 32 rows 15 / 22, 64 rows
+  // 30 / 21; 65536 columns 8 rows 23 / 26, 16 rows 40 / 22).  Clusters of 16
+  // lose to clusters of 4 with 32 keys whatever the rows (65540 columns 1 row
+  // 42 / 24; 131072 columns 1 row 42 / 24, 4 rows 43 / 25, 8 rows 85 / 25, 32
+  // rows 214 / 30): they are left to rows of more than 262144 columns.
+  const int at_once = C <= 4 ? num_sms() / 4 : num_sms() / 12;
+  if (C > 8 || (C >= 4 && p.rows > at_once)) {
     V = 32;
     C = pow2_ceil((w + kThreads * V - 1) / (kThreads * V));
   }

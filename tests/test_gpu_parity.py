@@ -103,6 +103,25 @@ def test_topk_expand_cluster_widths(dev, rows, width, topk):
         assert np.array_equal(counts, ref_counts)
 
 
+@pytest.mark.parametrize("rows,width,topk", [
+    (1, 262148, 512), (2, 400001, 4096), (1, 524288, 8192),   # clusters of 16, 32 keys a thread
+    (1, 262144, 512),                                         # of 8, 32 keys
+    (1, 65540, 512), (3, 100000, 2048), (5, 131072, 64),      # of 4, 32 keys
+    (36, 32768, 512), (38, 32768, 512),     # of 4 with 8 keys; of 1 with 32 once there are more
+    (12, 65536, 512), (13, 65536, 512),     # of 8 with 8 keys; of 2 with 32
+    (40, 16385, 512), (37, 16388, 16000),
+])
+def test_topk_expand_plans_by_width_and_rows(dev, rows, width, topk):
+    """Every cluster width, and both sides of the row counts where 32 keys a thread take over
+    from 8."""
+    for kind in ("relu", "ties"):
+        case = make_case(rows * 11 + width, rows, width, topk * 4, kind=kind, lengths="full")
+        got, counts = run_topk_expand(case, dev)
+        ref, ref_counts = oracle_topk_expand(case)
+        assert np.array_equal(got, ref), kind
+        assert np.array_equal(counts, ref_counts)
+
+
 @pytest.mark.parametrize("rows,width,token_topk", [(1779, 2048, 1024), (1803, 2000, 1200),
                                                    (1801, 2048, 4096), (1790, 1500, 4400),
                                                    (1777, 700, 0), (33, 2048, 1024),
