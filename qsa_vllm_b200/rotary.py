@@ -38,8 +38,10 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str =
     ``scaling``: "none"; "linear" (positions divided by ``scaling_factor``); "ntk" (the base
     grown so that the slowest pair is divided by it and the fastest unchanged); "yarn" (pairs
     that turn more than ``beta_fast`` times over ``original_length`` positions unchanged, those
-    that turn fewer than ``beta_slow`` times divided, a linear ramp over the number of turns
-    between them, and a factor of ``0.1 ln(scaling_factor) + 1``)."""
+    that turn fewer than ``beta_slow`` times divided, and a factor of ``0.1 ln(scaling_factor) +
+    1``).  Between them yarn's share of the division grows linearly with the pair's index, from
+    the last whole index at ``beta_fast`` turns to the first at ``beta_slow``, as in the code
+    that checkpoints are trained and served with (the paper's ramp is linear in the turns)."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
     if not (base > 0 and scaling_factor >= 1):
@@ -57,9 +59,16 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str =
             raise ValueError("yarn scaling needs original_length")
         if not beta_fast > beta_slow:
             raise ValueError("yarn scaling needs beta_fast > beta_slow")
-        turns = original_length * f / (2 * math.pi)
-        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0, 1)
-        f = f / scaling_factor * (1 - keep) + f * keep
+        if not base > 1 or not beta_slow > 0:
+            raise ValueError("yarn scaling needs a base above 1 and a positive beta_slow")
+
+        def index(turns):  # of the pair that turns so often, as a real number
+            return half * math.log(original_length / (2 * math.pi * turns)) / math.log(base)
+        last = min(math.ceil(index(beta_slow)), rotary_dim - 1)
+        first = min(max(math.floor(index(beta_fast)), 0), last)
+        # a ramp of no length is a step behind `first`
+        divided = ((i - first) / max(last - first, 0.001)).clamp(0, 1)
+        f = f / scaling_factor * divided + f * (1 - divided)
         factor = 0.1 * math.log(scaling_factor) + 1
     elif scaling not in ("none", "ntk"):
         raise ValueError(f"unknown scaling {scaling!r}")

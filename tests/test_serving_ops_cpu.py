@@ -284,3 +284,34 @@ def test_a_table_without_columns_is_not_in_place():
         got = _tables("cache_compact", -1, table, empty)
         assert got[3] and got[3] != got[0] and got[5] == 0
     assert _tables("cache_compact", -1, table, None)[3] is None
+
+
+@pytest.mark.parametrize("dim,base,length,factor,first,last", [
+    # indexes of the pairs that turn 32 times and once: 20.94 and 45.03; 38.99 and 63.07 of 64;
+    # 10.47 and 22.51 of 32; 11.97 and 68.67 of 64, whose ramp does not end within the head
+    (128, 10000.0, 4096, 4.0, 20, 46),
+    (128, 10000.0, 55000, 16.0, 38, 64),
+    (64, 10000.0, 4096, 4.0, 10, 23),
+    (128, 50.0, 418, 2.0, 11, 69),
+    (128, 10000.0, 6, 2.0, 0, 0),      # hardly a turn at all: only the first pair is kept
+    (128, 10000.0, 3, 2.0, -6, -5),    # not even that
+])
+def test_yarn_ramps_over_the_pairs(dim, base, length, factor, first, last):
+    """Between whole indexes of pairs the division sets in linearly with the index."""
+    from qsa_vllm_b200.rotary import rotary_frequencies
+    got, scale = rotary_frequencies(dim, base, scaling="yarn", scaling_factor=factor,
+                                    original_length=length)
+    for i in range(dim // 2):
+        plain = base ** (-2 * i / dim)
+        share = float(i > first) if first == last else min(max((i - first) / (last - first), 0), 1)
+        want = plain * (1 - share + share / factor)
+        assert math.isclose(float(got[i]), want, rel_tol=1e-12), (i, share)
+    assert math.isclose(scale, 0.1 * math.log(factor) + 1)
+
+
+def test_yarn_refusals():
+    from qsa_vllm_b200.rotary import rotary_frequencies
+    for bad in (dict(base=1.0), dict(beta_slow=0.0), dict(beta_slow=33.0), dict(original_length=0)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(64, **{**dict(scaling="yarn", scaling_factor=2.0,
+                                             original_length=4096), **bad})
