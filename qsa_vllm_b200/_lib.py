@@ -163,6 +163,20 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def workspace_of(what: str, workspace: torch.Tensor | None, need: int,
+                 like: torch.Tensor) -> torch.Tensor | None:
+    """The caller's workspace, checked, or a fresh one where it is None or holds less than
+    ``need`` bytes (None where none are needed)."""
+    if workspace is not None:
+        if workspace.device != like.device:
+            raise TypeError(f"{what}: workspace must be on {like.device}, got {workspace.device}")
+        if not workspace.is_contiguous():
+            raise ValueError(f"{what}: workspace must be contiguous")
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        return torch.empty(need, dtype=torch.uint8, device=like.device)
+    return workspace if need else None
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

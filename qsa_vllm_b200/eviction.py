@@ -215,8 +215,7 @@ def cache_evict(weights: torch.Tensor, seq_lens: torch.Tensor, block_table: torc
         return kept, lengths
     lib = _lib.load_library()
     need = lib.qsa_cache_evict_workspace_bytes(requests, shape[1], budget, sinks, recent)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=k_cache.device)
+    workspace = _lib.workspace_of(what, workspace, need, k_cache)
     with _lib.on_device(dev):
         status = lib.qsa_cache_evict(
             weights.data_ptr(), ws[0], ws[1], shape[1], shape[2], seq_lens.data_ptr(), requests,

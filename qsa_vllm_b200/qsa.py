@@ -75,8 +75,7 @@ def qsa_sparse_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     hkv = k_cache.shape[2]
     width = logical_indices.shape[1]
     need = attention_workspace_bytes(rows, hq, hkv, d, width, use_decode_kernel)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    workspace = _lib.workspace_of("qsa_sparse_paged_attention", workspace, need, q)
     lib = _lib.load_library()
     with torch.cuda.device(q.device):
         _lib.check(lib.qsa_sparse_attention(

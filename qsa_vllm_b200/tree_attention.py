@@ -122,8 +122,7 @@ def tree_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     with _lib.on_device(index):
         need = lib.qsa_tree_attention_workspace_bytes(rows, tables[6], hq, tables[2], d,
                                                       max_query_len)
-        if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        workspace = _lib.workspace_of(what, workspace, need, q)
         status = lib.qsa_tree_attention(
             q.data_ptr(), qs[0], qs[1], rows, hq, d, _DTYPES[q.dtype], *keys, *values, *tables,
             d ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1],

@@ -315,3 +315,20 @@ def test_yarn_refusals():
         with pytest.raises(ValueError):
             rotary_frequencies(64, **{**dict(scaling="yarn", scaling_factor=2.0,
                                              original_length=4096), **bad})
+
+
+def test_workspaces_are_checked():
+    from qsa_vllm_b200._lib import workspace_of
+    like, ws = torch.zeros(1), torch.zeros(100, dtype=torch.uint8)
+    assert workspace_of("op", ws, 100, like) is ws
+    assert workspace_of("op", ws.view(torch.float32), 100, like).numel() == 25
+    assert workspace_of("op", ws, 101, like).numel() == 101   # too small: a fresh one
+    assert workspace_of("op", None, 7, like).numel() == 7
+    assert workspace_of("op", None, 0, like) is None and workspace_of("op", ws, 0, like) is None
+    for need in 100, 0:
+        with pytest.raises(TypeError, match="workspace"):
+            workspace_of("op", ws.to("meta"), need, like)
+        with pytest.raises(ValueError, match="workspace"):
+            workspace_of("op", ws[:1].expand(100), need, like)
+        with pytest.raises(ValueError, match="workspace"):
+            workspace_of("op", torch.zeros(200, dtype=torch.uint8)[::2], need, like)

@@ -178,3 +178,27 @@ def test_speculative_steps(dev, hq, hkv, d, page, steps, captured):
                     1 + w_new[h].max())
                 assert (w_final[h, now:total] == 0).all()
     assert _lib.device_error_poll() == 0
+
+
+def test_workspaces_of_another_device_are_refused(dev):
+    """A host address, or one byte for all, does not go to a kernel."""
+    from qsa_vllm_b200.eviction import cache_evict
+    from qsa_vllm_b200.qsa import qsa_sparse_paged_attention
+    from qsa_vllm_b200.tree_attention import tree_paged_attention
+    kv = torch.zeros(4, 16, 2, 256, dtype=torch.bfloat16, device=dev)
+    k, v = kv[..., :128], kv[..., 128:]
+    table = torch.arange(4, dtype=torch.int32, device=dev).view(1, 4)
+    lens = torch.full((1,), 60, dtype=torch.int32, device=dev)
+    start = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    q = torch.zeros(1, 8, 128, dtype=torch.bfloat16, device=dev)
+    idx = torch.arange(32, dtype=torch.int32, device=dev).view(1, 32)
+    w = torch.zeros(1, 2, 64, device=dev)
+    host = torch.empty(1 << 25, dtype=torch.uint8)
+    one = torch.empty(1, dtype=torch.uint8, device=dev).expand(1 << 25)
+    for ws, err in (host, TypeError), (one, ValueError):
+        with pytest.raises(err, match="workspace"):
+            tree_paged_attention(q, k, v, table, lens, start, max_query_len=1, workspace=ws)
+        with pytest.raises(err, match="workspace"):
+            cache_evict(w, lens, table, k, v, 40, workspace=ws)
+        with pytest.raises(err, match="workspace"):
+            qsa_sparse_paged_attention(q, k, v, idx, table, start[:1], workspace=ws)
