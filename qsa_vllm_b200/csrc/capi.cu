@@ -946,7 +946,7 @@ static int tree_common(TreeParams& p, const char* who, const void* q, int64_t q_
     return fail(QSA_ERR_INVALID, "%s: null pointer", who);
   if (!aligned(k_cache, 16) || k_block_stride % 8 || k_token_stride % 8 || k_head_stride % 8)
     return fail(QSA_ERR_INVALID, "%s: cache rows must be 16-byte aligned", who);
-  if (!aligned(q, 16) || q_row_stride % 8 || q_head_stride % 8)
+  if (rows > 0 && (!aligned(q, 16) || q_row_stride % 8 || q_head_stride % 8))
     return fail(QSA_ERR_INVALID, "%s: q head rows must be 16-byte aligned", who);
   p.q = q;
   p.q_row_stride = q_row_stride;

@@ -332,3 +332,18 @@ def test_workspaces_are_checked():
             workspace_of("op", ws[:1].expand(100), need, like)
         with pytest.raises(ValueError, match="workspace"):
             workspace_of("op", torch.zeros(200, dtype=torch.uint8)[::2], need, like)
+
+
+def test_weights_without_rows_take_any_strides_of_q():
+    """A slice without rows of an unaligned projection has nothing to align (a capacity of 0:
+    behind the checks nothing is launched)."""
+    from qsa_vllm_b200 import _lib
+    lib = _lib.load_library()
+
+    def weights(rows, q, head):
+        return lib.qsa_attention_weights(
+            q, 4 * head, head, rows, 4, 64, 0, 4096, 64, 64, 64, 8, 16, 2, 4096, 4, 4, 2, 4096,
+            4096, None, 0, 0, 1, 0.125, 4096, 4, None, 0, 4096, 0, 0, 4096, 0, 0, 0, None)
+    assert weights(0, None, 67) == 0 and weights(0, 4098, 67) == 0 and weights(3, 4096, 64) == 0
+    for bad in (3, 4098, 64), (3, 4096, 67), (3, None, 64):
+        assert weights(*bad) == 1, bad
