@@ -447,8 +447,10 @@ QSA_API size_t qsa_tree_attention_workspace_bytes(int32_t rows, int32_t num_requ
  * page_size, num_kv_heads, head_dim]; bf16 or fp16, unit dim strides, 16-byte
  * aligned rows of q and caches.  head_dim a multiple of 8 up to 256; head_dim
  * 64 / 128 with pages that are a multiple of 8 run on the tensor cores.
- * max_query_len sizes the work split (the longest request's rows; a smaller
- * value costs speed, not results).  table_width * page_size at most 2^30.
+ * max_query_len sizes the work split, not the results: the longest request's
+ * rows, or in a batch of single rows beside a few prompt chunks 1 (the longest
+ * chunk's rows take 4 times as long there).  table_width * page_size at most
+ * 2^30.
  */
 QSA_API int qsa_tree_attention(
     const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t rows, int32_t num_q_heads,
@@ -491,6 +493,10 @@ QSA_API int qsa_attention_weights(
 /*
  * Compaction of cached tokens.  No counterpart in the reference.
  *
+ * For caches of dense layers, as is qsa_cache_evict: of a QSA layer only the
+ * keys and values would move, and its compressed index keys (qsa_prepare)
+ * would describe the tokens that were there before.
+ *
  * For every request b, KV head h and j < count with indices[b, h, j] >= 0, the
  * key and value rows of logical token indices[b, h, j] go to logical token
  * starts[b] + j (starts NULL: j).  Entries below 0 move nothing.  Tokens are
@@ -532,7 +538,8 @@ QSA_API size_t qsa_cache_evict_workspace_bytes(int32_t num_requests, int32_t lis
  * The kept tokens, ascending, become tokens 0 .. min(L, budget) - 1: their K/V
  * rows move as qsa_cache_compact moves them (in place, or to out_table's
  * pages), weights_out[b, h, j] = weights[b, h, kept[j]], zero from there to L
- * (entries from L on are not written).  kept [num_requests, list_heads,
+ * (entries from L on are not written).  Kept tokens outside a table or on
+ * unmapped pages are skipped as there.  kept [num_requests, list_heads,
  * budget] receives the old token numbers, -1 behind the last; lengths_out
  * [num_requests] the new lengths.  seq_lens is not written, and neither
  * weights_out unless it is weights may overlap what the call reads.

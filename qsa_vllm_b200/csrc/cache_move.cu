@@ -19,8 +19,13 @@
 // token of a group finds its source and destination and leaves their offsets
 // in shared memory, where the threads that copy 16 bytes at a time pick them
 // up: found by every copying thread for itself they cost more instructions
-// than the memory leaves time for (464 instead of
-// 180 us for 1.07 GB of rows, whose floor at a copy's rate is 164).
+// than the memory leaves time for (464 instead of 180 us for 1.07 GB of rows
+// to other pages, whose floor at a copy's rate is 164).  In place a round at a
+// time is in flight, and the number of CTAs in a cluster decides (us for 1 / 2
+// / 4 / 8: 32 lists that keep 8192 of 33k to 131k tokens 452 / 373 / 211 / 128,
+// 64 lists of 8191 rows 336 / 232 / 150 / 103, floor 82), as long as the lists
+// alone do not fill the GPU (512 lists of 2048 tokens 120 / 132 / 132 / 132,
+// the rule's choice being 2).
 #include <algorithm>
 
 #include "common.cuh"

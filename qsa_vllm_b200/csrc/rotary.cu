@@ -22,8 +22,13 @@
 // that a head costs little more than its loads, products and stores: finding
 // (token, head, chunk) anew for every 16 bytes was instruction-bound (39 us
 // instead of 19.5 us for 8192 tokens of 20 heads).  What is only copied (dims
-// past the rotated ones, values) follows.  Bound by memory: each value is read
-// and written once.
+// past the rotated ones, values) follows.
+//
+// Each value is read and written once: 8192 tokens of 16 + 2 + 2 heads of 128,
+// interleaved, would take 12.9 us at a copy's rate, and torch's elementwise
+// kernel takes 14.5 us for as many bytes.  The interleaved 16-bit form, held to
+// 64 registers for 8 blocks an SM, spills 24 bytes a thread, which is likely a
+// part of what lies between that and its 19.5 us; the others do not spill.
 #include <cuda_fp16.h>
 
 #include <algorithm>

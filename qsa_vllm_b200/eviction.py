@@ -13,6 +13,11 @@ Attention does not depend on the order or the numbering of cached tokens: keys k
 positions they were stored with.  After an eviction the tokens' numbers are new ones, so the
 caller goes on counting positions for itself, frees the pages behind the new lengths, and
 appends at the new length.
+
+These are operators for layers with dense attention.  The cache of a QSA layer must not be passed:
+only its keys and values would move, while its compressed index keys and its ring of raw ones,
+which ``qsa_prepare`` wrote, would go on describing the tokens that were there before.  Its sparse
+attention leaves no log-sum-exp over all tokens either.
 """
 
 from __future__ import annotations
@@ -81,7 +86,8 @@ def accumulate_attention_weights(
     Arguments as in ``tree_paged_attention``, whose ``lse`` this takes.  row_factors: fp32
     ``[rows]``, 1 where None; 0 leaves a row out (a rejected draft).  weights, out: fp32 ``[B,
     H_kv, capacity]``; out is weights itself (in place) where None.  Tokens from
-    ``min(seq_lens[b], capacity)`` on are not written."""
+    ``min(seq_lens[b], capacity, width * page)`` on (past the lengths, the capacity or the block
+    table) are not written; tokens on unmapped pages keep their weight."""
     what = "accumulate_attention_weights"
     keys, _, tables = check_tree_arguments(what, q, k_cache, None, block_table, seq_lens,
                                            query_start_loc, tree_mask, max_query_len)

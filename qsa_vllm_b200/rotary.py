@@ -12,7 +12,8 @@ For pair ``i`` of a token at position ``p``, with ``a = p * frequencies[i]``::
 
 ``(x1, x2)`` are ``x[i], x[i + rotary_dim / 2]``, or ``x[2i], x[2i + 1]`` when
 ``interleaved``; dims from ``rotary_dim`` on pass through.  Angles are formed and reduced
-in 64 bits, so positions of any size keep their precision; no table is kept.
+in 64 bits, to within 2^-24 of a turn up to position 2^30 (and with 2^-54 of the position
+beyond); no table is kept.
 ``inverse=True`` turns back, and with the same ``factor`` is the operator's gradient:
 ``dx = rotary_embed(dy, ..., inverse=True)``.
 """

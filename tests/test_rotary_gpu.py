@@ -229,3 +229,29 @@ def test_captured_and_replayed_on_another_stream(dev):
     torch.cuda.current_stream().wait_stream(side)
     want = rotary_embed(q, k, pos, freq)
     assert torch.equal(qo, want[0]) and torch.equal(ko, want[1])
+
+
+def test_positions_past_what_64_bits_hold_exactly(dev):
+    """Positions up to 2^52, against angles reduced with 60 decimal digits: a turn is off by at
+    most 2^-54 of the position (two products and the constant 1 / 2 pi, each rounded to 2^-53 of
+    position / 2 pi) and by 2^-25 for its 32-bit form; sine and cosine by 2 pi times that and two
+    units of their own; y1 and y2 are a sum of two products of values up to 1."""
+    import math
+    from decimal import Decimal, getcontext
+    from qsa_vllm_b200.rotary import rotary_embed, rotary_frequencies
+    getcontext().prec = 60
+    two_pi = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781")
+    freq, _ = rotary_frequencies(32)
+    pos = torch.tensor([1, 3, 4095, 2**20 + 1, 2**30 - 1, 2**33 + 5, 2**40 - 3, 2**45 + 77, 2**52])
+    pos = torch.cat([pos, -pos])
+    q = torch.ones(pos.numel(), 1, 32, device=dev)
+    y, _ = rotary_embed(q, None, pos.to(dev), freq.to(dev))
+    y = y.double().cpu()[:, 0]
+    for n, at in enumerate(pos.tolist()):
+        for i, f in enumerate(freq.tolist()):
+            turns = Decimal(at) * Decimal(f) / two_pi
+            a = 2 * math.pi * float(turns - turns.to_integral_value())
+            off = 2 * math.pi * (abs(at) * f * 2.0 ** -54 + 2.0 ** -25) + 2 * 2.0 ** -24
+            c, s = math.cos(a), math.sin(a)
+            assert abs(y[n, i] - (c - s)) <= 2 * off + 3 * 2.0 ** -24, (at, i)
+            assert abs(y[n, i + 16] - (c + s)) <= 2 * off + 3 * 2.0 ** -24, (at, i)
