@@ -100,9 +100,9 @@ def tree_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     tokens]``, nonzero where the row sees its request's drafted token (itself too); None for a
     chain.  scale: ``d ** -0.5`` where None.  lse: fp32 ``[rows, H_q]``, receives the natural
     log-sum-exp.  max_query_len: the longest request's rows (a host number that sizes the work
-    split, and changes nothing else); 1 in a batch of single rows beside a few prompt chunks,
-    which would all be split as the chunks are (63 rows and a chunk of 512 over 8192 tokens: 259
-    us with 1, 1026 with 512).  Rows that see nothing give 0 and -inf; rows of no request are left
+    split, and through it the order of 32-bit sums); 1 in a batch of single rows beside a few
+    prompt chunks, which would all be split as the chunks are (63 rows and a chunk of 512 over
+    8192 tokens: 259 us with 1, 1026 with 512).  Rows that see nothing give 0 and -inf; rows of no request are left
     as they are.
     workspace: uint8, at least ``tree_attention_workspace_bytes(...)``; allocated where None."""
     what = "tree_paged_attention"
